@@ -66,6 +66,9 @@ _SIGNATURES = {
     "mi_decoder_read": (_i, [_vp, _vp, C.POINTER(_i), C.POINTER(_i)]),
     "mi_decoder_logits": (_vp, [_vp]),
     "mi_decoder_buffer": (_vp, [_vp, _i]),
+    "mi_kv_write": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i]),
+    "mi_kv_read": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i]),
+    "mi_attention": (_i, [_vp, _vp]),
     "mi_argmax_f16": (_i, [_vp, _vp, _i, _i, _vp]),
     "mi_linear_argmax": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
     "mi_linear_argmax_static": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
@@ -390,6 +393,64 @@ class Decoder:
 
     def __del__(self):
         self.close()
+
+
+# ------------------------------------------- attention over a cache in pages (include/mi_attention.h)
+
+KV_F16, KV_INT8, KV_Q4 = 0, 8, 4
+
+
+class KVCache(C.Structure):
+    """mi_kv_cache: the pools of one layer's keys and values, [n_pages, n_kv_heads, page_size, row], and for int8 and Q4
+    their fp16 scales.  k, v, k_scale, v_scale: Buffers or device addresses."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)] + \
+               [(n, _i) for n in ("kind", "n_pages", "page_size", "n_kv_heads", "head_dim")]
+
+    def __init__(self, kind, n_pages, page_size, n_kv_heads, head_dim, k, v, k_scale=None, v_scale=None):
+        super().__init__(_h(k), _h(v), _h(k_scale), _h(v_scale), kind, n_pages, page_size, n_kv_heads, head_dim)
+        self._keep = (k, v, k_scale, v_scale)
+
+
+class KVBatch(C.Structure):
+    """mi_kv_batch: the sequences of a call.  q_start [n_seqs + 1], kv_len [n_seqs], pages [n_seqs, max_pages]: int32 in
+    device memory; n_tokens rows, of which a sequence has at most max_tokens (a hint)."""
+    _fields_ = [("q_start", _vp), ("kv_len", _vp), ("pages", _vp)] + \
+               [(n, _i) for n in ("n_seqs", "n_tokens", "max_tokens", "max_pages")]
+
+    def __init__(self, n_seqs, n_tokens, max_tokens, max_pages, q_start, kv_len, pages):
+        super().__init__(_h(q_start), _h(kv_len), _h(pages), n_seqs, n_tokens, max_tokens, max_pages)
+        self._keep = (q_start, kv_len, pages)
+
+
+class AttentionCall(C.Structure):
+    """mi_attention_call: a prepared call of attention().  ld_q, ld_out: elements from row to row (0: n_heads * head_dim);
+    scale: None for 1 / sqrt(head_dim)."""
+    _fields_ = [("cache", C.POINTER(KVCache)), ("batch", C.POINTER(KVBatch)), ("q", _vp), ("out", _vp), ("ld_q", _i),
+                ("ld_out", _i), ("n_heads", _i), ("scale", C.c_float), ("window", _i), ("sinks", _i)]
+
+    def __init__(self, cache, batch, n_heads, q, out, ld_q=0, ld_out=0, scale=None, window=0, sinks=0):
+        width = n_heads * cache.head_dim
+        super().__init__(C.pointer(cache), C.pointer(batch), _h(q), _h(out), ld_q or width, ld_out or width, n_heads,
+                         cache.head_dim ** -0.5 if scale is None else scale, window, sinks)
+        self._keep = (cache, batch, q, out)
+
+
+def kv_write(queue, cache, batch, k, v, ld_k=0, ld_v=0):
+    """New tokens' keys and values into their pages (mi_kv_write); ld_k, ld_v: 0 for n_kv_heads * head_dim."""
+    width = cache.n_kv_heads * cache.head_dim
+    return bool(lib().mi_kv_write(_q(queue), C.addressof(cache), C.addressof(batch), _h(k), ld_k or width, _h(v), ld_v or width))
+
+
+def kv_read(queue, cache, batch, k_out, v_out, ld_k=0, ld_v=0):
+    """The same rows back out of their pages, as fp16 (mi_kv_read)."""
+    width = cache.n_kv_heads * cache.head_dim
+    return bool(lib().mi_kv_read(_q(queue), C.addressof(cache), C.addressof(batch), _h(k_out), ld_k or width, _h(v_out),
+                                 ld_v or width))
+
+
+def attention(queue, call):
+    """Attention of the new tokens over the cache (mi_attention)."""
+    return bool(lib().mi_attention(_q(queue), C.addressof(call)))
 
 
 # ------------------------------------------------------------------- offline tools

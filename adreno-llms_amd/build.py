@@ -9,7 +9,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmi_linear.so")
-SOURCES = ["runtime.hip", "gemv.hip", "gemm.hip", "argmax.hip", "decode.hip", "attention.hip", "probe.hip", "quantize.cpp", "bundle.cpp"]
+SOURCES = ["runtime.hip", "gemv.hip", "gemm.hip", "argmax.hip", "decode.hip", "attention.hip", "kv_cache.hip",
+           "paged_attention.hip", "probe.hip", "quantize.cpp", "bundle.cpp"]
 
 # -ffp-contract=off: the kernels spell every fused multiply-add as fmaf(); nothing else
 # may be fused, or results stop being bit-identical to the reference evaluation order.

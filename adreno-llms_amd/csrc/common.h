@@ -126,6 +126,8 @@ WeightEntry weight_entry(const void* W);
 uint64_t registry_epoch();
 // The workspace of a stream that mi_stream_create made (null: another stream, or no memory was left for one)
 void* own_stream_workspace(hipStream_t s);
+// The same, of the null stream as well
+void* stream_workspace(hipStream_t s);
 // While it lives, launches that this thread enqueues on `recording` (a stream of the library's own, under capture) use the
 // workspace and the modes of `s`, the stream that the recording will be replayed on.  One at a time in a thread.
 class StandsFor {

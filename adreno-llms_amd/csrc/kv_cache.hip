@@ -1,0 +1,305 @@
+// Rows of keys and values into the pages of a cache and back out (mi_kv_write, mi_kv_read), and the checks that the entry
+// points over such a cache share.  The reference appends one row at the sequence's position, fp16 (KV cache
+// QW/src/layers/attention.cpp:111-131).
+//
+// scale = fp16(greatest |x| / top) with top = 127 or 7, code = x / scale to the nearest integer, ties to even.  Both are
+// exact: an fp16 number over 127 or 7 is never within 2^-9 of an fp16 step of the middle between two fp16 numbers, and a quotient of
+// two fp16 numbers that is not a half-integer is at least 2^-12 away from one, more than the fp32 division's error at 127.
+#include "../../include/mi_linear.h"
+#include "device_math.h"
+#include "paged.h"
+
+#include <cmath>
+
+namespace mi {
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256;
+constexpr int kPiece = 8;                          // values per thread: 16 bytes of an fp16 row
+
+// Where a thread's 8 values are: row of the batch, head, first element, and the row's number in the pools (-1: it has no place).
+struct Place {
+    int row, head, at;
+    int64_t cache;
+    bool mine;                                     // the row belongs to a sequence
+};
+template <int D>
+__device__ __forceinline__ Place place_of(const PagedArgs& a) {
+    constexpr int kPieces = D / kPiece;
+    const int64_t id = static_cast<int64_t>(blockIdx.x) * (kThreads / kPieces) + threadIdx.x / kPieces;
+    Place p{};
+    p.cache = -1;
+    p.row = static_cast<int>(id / a.n_kv_heads);
+    p.head = static_cast<int>(id % a.n_kv_heads);
+    p.at = static_cast<int>(threadIdx.x % kPieces) * kPiece;
+    if (p.row >= a.n_tokens) return p;
+    const int b = sequence_of(a.q_start, a.n_seqs, p.row);
+    if (b < 0) return p;
+    const Span s = span_of(a.q_start[b], a.q_start[b + 1], a.kv_len[b], a.n_tokens);
+    if (p.row - s.first >= s.n) return p;
+    p.mine = true;
+    const int pos = s.pos + (p.row - s.first);
+    if (pos < 0 || pos >= a.cap) return p;
+    const int page = divide(pos, a.page);
+    const int number = a.pages[static_cast<int64_t>(b) * a.max_pages + page];
+    if (number < 0 || number >= a.n_pages) return p;
+    p.cache = row_number(a, number, p.head, pos - page * a.page.d);
+    return p;
+}
+
+// The greatest of the values of N neighbouring lanes (N = 4, 8, 16: a piece of a DPP row), in each of them.
+template <int N>
+__device__ __forceinline__ float max_of(float m) {
+    m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xb1, 0xf, 0xf, true)));     // lane ^ 1
+    m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4e, 0xf, 0xf, true)));     // lane ^ 2
+    if constexpr (N >= 8) m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x141, 0xf, 0xf, true)));  // half row mirrored
+    if constexpr (N >= 16) m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x140, 0xf, 0xf, true))); // row mirrored
+    return m;
+}
+
+// blockIdx.y: keys, values.  Bound by bytes where there are many rows (16 in and 16, 8 or 4 out per thread), by the chain
+// of loads to a row's place (q_start, kv_len, pages) where there are few.
+template <int KIND, int D>
+__global__ __launch_bounds__(kThreads) void kv_write_kernel(const PagedArgs a, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
+                                                            const int64_t ld_k, const int64_t ld_v) {
+    const Place p = place_of<D>(a);
+    if (p.cache < 0) return;                       // (all lanes of a row alike)
+    const uint16_t* src = blockIdx.y ? v + p.row * ld_v : k + p.row * ld_k;
+    src += p.head * D + p.at;
+    half8 x;
+    if (reinterpret_cast<uintptr_t>(src) % 16 == 0) x = *reinterpret_cast<const half8*>(src);
+    else
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(_Float16, src[e]);
+    uint8_t* const pool = const_cast<uint8_t*>(blockIdx.y ? a.v : a.k);
+    if constexpr (KIND == MI_KV_F16) {
+        *reinterpret_cast<half8*>(pool + (p.cache * D + p.at) * 2) = x;
+    } else {
+        constexpr bool kInt8 = KIND == MI_KV_INT8;
+        constexpr float kTop = kInt8 ? 127.0f : 7.0f, kMost = kInt8 ? 515.5f : 9352.0f;     // (code * scale stays below 65520)
+        // 0 for all finite values, else NaN: a NaN would be lost among maxima
+        float big = 0.0f, bad = 0.0f;
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float f = static_cast<float>(x[e]);
+            big = fmaxf(big, fabsf(f));
+            bad += f * 0.0f;
+        }
+        if (bad != 0.0f) big = __builtin_huge_valf();
+        big = max_of<kInt8 ? D / kPiece : 32 / kPiece>(big);
+        const bool finite = big <= 65504.0f;
+        const _Float16 h = static_cast<_Float16>(finite ? fminf(__fdiv_rn(big, kTop), kMost) : __builtin_nanf(""));
+        const float scale = static_cast<float>(h);
+        int code[8];
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float c = finite && scale > 0.0f ? rintf(__fdiv_rn(static_cast<float>(x[e]), scale)) : 0.0f;
+            code[e] = static_cast<int>(fminf(fmaxf(c, kInt8 ? -127.0f : -8.0f), kTop));
+        }
+        uint16_t* const scales = const_cast<uint16_t*>(blockIdx.y ? a.v_scale : a.k_scale);
+        if constexpr (kInt8) {
+            u32x2 w = {0, 0};
+            #pragma unroll
+            for (int e = 0; e < 8; ++e) w[e / 4] |= static_cast<uint32_t>(code[e] & 255) << (8 * (e % 4));
+            *reinterpret_cast<u32x2*>(pool + p.cache * D + p.at) = w;
+            if (p.at == 0) scales[p.cache] = __builtin_bit_cast(uint16_t, h);
+        } else {
+            uint32_t w = 0;
+            #pragma unroll
+            for (int e = 0; e < 8; ++e) w |= static_cast<uint32_t>(code[e] + 8) << (4 * e);
+            *reinterpret_cast<uint32_t*>(pool + (p.cache * D + p.at) / 2) = w;
+            if (p.at % 32 == 0) scales[p.cache * (D / 32) + p.at / 32] = __builtin_bit_cast(uint16_t, h);
+        }
+    }
+}
+
+template <int KIND, int D>
+__global__ __launch_bounds__(kThreads) void kv_read_kernel(const PagedArgs a, uint16_t* __restrict__ k, uint16_t* __restrict__ v,
+                                                           const int64_t ld_k, const int64_t ld_v) {
+    const Place p = place_of<D>(a);
+    if (!p.mine) return;
+    half8 x;
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = static_cast<_Float16>(0.0f);
+    if (p.cache >= 0) {
+        const uint8_t* const pool = blockIdx.y ? a.v : a.k;
+        if constexpr (KIND == MI_KV_F16) {
+            x = *reinterpret_cast<const half8*>(pool + (p.cache * D + p.at) * 2);
+        } else {
+            const uint16_t* const scales = blockIdx.y ? a.v_scale : a.k_scale;
+            if constexpr (KIND == MI_KV_INT8) {
+                const float scale = h_f(scales[p.cache]);
+                const u32x2 w = *reinterpret_cast<const u32x2*>(pool + p.cache * D + p.at);
+                #pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] = static_cast<_Float16>(static_cast<float>(static_cast<int8_t>(w[e / 4] >> (8 * (e % 4)))) * scale);
+            } else {
+                const float scale = h_f(scales[p.cache * (D / 32) + p.at / 32]);
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(pool + (p.cache * D + p.at) / 2);
+                #pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] = static_cast<_Float16>(static_cast<float>(static_cast<int>(w >> (4 * e) & 15) - 8) * scale);
+            }
+        }
+    }
+    uint16_t* dst = blockIdx.y ? v + p.row * ld_v : k + p.row * ld_k;
+    dst += p.head * D + p.at;
+    if (reinterpret_cast<uintptr_t>(dst) % 16 == 0) *reinterpret_cast<half8*>(dst) = x;
+    else
+        #pragma unroll
+        for (int e = 0; e < 8; ++e) dst[e] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e]));
+}
+
+// Blocks for one thread per 8 values of a row of keys; 0: more than a grid counts.
+unsigned blocks_for(const PagedArgs& a, int D) {
+    const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.n_kv_heads, per_block = kThreads / (D / kPiece);
+    const int64_t blocks = (rows + per_block - 1) / per_block;
+    return blocks > 0x7fffffff / kThreads ? 0u : static_cast<unsigned>(blocks);
+}
+
+bool bad_rows(const char* who, const void* k, int ld_k, const void* v, int ld_v, const PagedArgs& a, int D) {
+    const int64_t width = static_cast<int64_t>(a.n_kv_heads) * D;
+    if (k && v && ld_k >= width && ld_v >= width && reinterpret_cast<uintptr_t>(k) % 2 == 0 && reinterpret_cast<uintptr_t>(v) % 2 == 0)
+        return false;
+    MI_ERROR_FMT("%s: bad rows (k=%p ld_k=%d v=%p ld_v=%d, %lld elements each)", who, k, ld_k, v, ld_v, static_cast<long long>(width));
+    return true;
+}
+
+}  // namespace
+
+bool paged_args(const char* who, const mi_kv_cache* c, const mi_kv_batch* b, PagedArgs* out) {
+    if (!c || !b) {
+        MI_ERROR_FMT("%s: null cache or batch", who);
+        return false;
+    }
+    const bool quantised = c->kind == MI_KV_INT8 || c->kind == MI_KV_Q4;
+    if ((c->kind != MI_KV_F16 && !quantised) || (c->head_dim != 64 && c->head_dim != 128) || c->n_pages < 1 || c->page_size < 1 ||
+        c->n_kv_heads < 1) {
+        MI_ERROR_FMT("%s: bad cache (kind=%d n_pages=%d page_size=%d n_kv_heads=%d head_dim=%d)", who, c->kind, c->n_pages,
+                     c->page_size, c->n_kv_heads, c->head_dim);
+        return false;
+    }
+    const auto off = [](const void* p, uintptr_t align) { return !p || reinterpret_cast<uintptr_t>(p) % align; };
+    if (off(c->k, 16) || off(c->v, 16) || (quantised && (off(c->k_scale, 8) || off(c->v_scale, 8)))) {
+        MI_ERROR_FMT("%s: pools must be 16-byte aligned, scales 8-byte (k=%p v=%p k_scale=%p v_scale=%p)", who, c->k, c->v, c->k_scale,
+                     c->v_scale);
+        return false;
+    }
+    const double page_bytes = static_cast<double>(c->n_kv_heads) * c->page_size * row_bytes(c->kind, c->head_dim);
+    if (page_bytes >= 2147483648.0) {
+        MI_ERROR_FMT("%s: a page of %.0f bytes (less than 2 GiB are taken)", who, page_bytes);
+        return false;
+    }
+    if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_pages < 1 ||
+        (b->n_seqs > 0 && (off(b->q_start, 4) || off(b->kv_len, 4) || off(b->pages, 4)))) {
+        MI_ERROR_FMT("%s: bad batch (n_seqs=%d n_tokens=%d max_pages=%d q_start=%p kv_len=%p pages=%p)", who, b->n_seqs, b->n_tokens,
+                     b->max_pages, static_cast<const void*>(b->q_start), static_cast<const void*>(b->kv_len),
+                     static_cast<const void*>(b->pages));
+        return false;
+    }
+    PagedArgs a{};
+    a.k = static_cast<const uint8_t*>(c->k);
+    a.v = static_cast<const uint8_t*>(c->v);
+    a.k_scale = static_cast<const uint16_t*>(c->k_scale);
+    a.v_scale = static_cast<const uint16_t*>(c->v_scale);
+    a.q_start = b->q_start;
+    a.kv_len = b->kv_len;
+    a.pages = b->pages;
+    a.n_seqs = b->n_seqs;
+    a.n_tokens = b->n_tokens;
+    a.max_pages = b->max_pages;
+    a.n_pages = c->n_pages;
+    a.n_kv_heads = c->n_kv_heads;
+    a.cap = capacity(b->max_pages, c->page_size);
+    a.page = make_divider(c->page_size);
+    *out = a;
+    return true;
+}
+
+#define MI_KV_LAUNCH(KERNEL, K, V)                                                                                                   \
+    [&] {                                                                                                                            \
+        const dim3 grid(blocks, 2), block(kThreads);                                                                                 \
+        const auto s = static_cast<hipStream_t>(stream);                                                                             \
+        auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, s, a, K, V, ld_k, ld_v); };                              \
+        const bool wide = cache->head_dim == 128;                                                                                    \
+        if (cache->kind == MI_KV_F16) wide ? go(KERNEL<MI_KV_F16, 128>) : go(KERNEL<MI_KV_F16, 64>);                                 \
+        else if (cache->kind == MI_KV_INT8) wide ? go(KERNEL<MI_KV_INT8, 128>) : go(KERNEL<MI_KV_INT8, 64>);                         \
+        else wide ? go(KERNEL<MI_KV_Q4, 128>) : go(KERNEL<MI_KV_Q4, 64>);                                                            \
+        return MI_HIP_OK(hipGetLastError()) ? 1 : 0;                                                                                 \
+    }()
+
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" int mi_kv_write(void* stream, const mi_kv_cache* cache, const mi_kv_batch* batch, const void* k, int ld_k, const void* v, int ld_v) {
+    PagedArgs a;
+    if (!paged_args("mi_kv_write", cache, batch, &a) || bad_rows("mi_kv_write", k, ld_k, v, ld_v, a, cache->head_dim)) return 0;
+    if (a.n_seqs == 0 || a.n_tokens == 0) return 1;
+    const unsigned blocks = blocks_for(a, cache->head_dim);
+    if (!blocks) {
+        MI_ERROR_FMT("mi_kv_write: %d rows of %d heads are more than a launch counts", a.n_tokens, a.n_kv_heads);
+        return 0;
+    }
+    if (!ensure_init()) return 0;
+    return MI_KV_LAUNCH(kv_write_kernel, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v));
+}
+
+extern "C" int mi_kv_read(void* stream, const mi_kv_cache* cache, const mi_kv_batch* batch, void* k, int ld_k, void* v, int ld_v) {
+    PagedArgs a;
+    if (!paged_args("mi_kv_read", cache, batch, &a) || bad_rows("mi_kv_read", k, ld_k, v, ld_v, a, cache->head_dim)) return 0;
+    if (a.n_seqs == 0 || a.n_tokens == 0) return 1;
+    const unsigned blocks = blocks_for(a, cache->head_dim);
+    if (!blocks) {
+        MI_ERROR_FMT("mi_kv_read: %d rows of %d heads are more than a launch counts", a.n_tokens, a.n_kv_heads);
+        return 0;
+    }
+    if (!ensure_init()) return 0;
+    return MI_KV_LAUNCH(kv_read_kernel, static_cast<uint16_t*>(k), static_cast<uint16_t*>(v));
+}
+
+extern "C" int mi_attention(void* stream, const mi_attention_call* call) {
+    if (!call) {
+        MI_ERROR_FMT("mi_attention: null call");
+        return 0;
+    }
+    const mi_attention_call& c = *call;
+    PagedArgs p;
+    if (!paged_args("mi_attention", c.cache, c.batch, &p)) return 0;
+    const int64_t width = static_cast<int64_t>(c.n_heads) * c.cache->head_dim;
+    if (c.n_heads < 1 || c.n_heads % p.n_kv_heads || !c.q || !c.out || c.ld_q < width || c.ld_out < width ||
+        reinterpret_cast<uintptr_t>(c.q) % 2 || reinterpret_cast<uintptr_t>(c.out) % 2) {
+        MI_ERROR_FMT("mi_attention: bad argument (n_heads=%d over %d q=%p ld_q=%d out=%p ld_out=%d)", c.n_heads, p.n_kv_heads, c.q, c.ld_q,
+                     c.out, c.ld_out);
+        return 0;
+    }
+    if (!(c.scale > 0.0f && c.scale <= 65504.0f) || c.sinks < 0) {
+        MI_ERROR_FMT("mi_attention: bad argument (scale=%g, window=%d, sinks=%d)", static_cast<double>(c.scale), c.window, c.sinks);
+        return 0;
+    }
+    if (p.n_seqs == 0 || p.n_tokens == 0) return 1;
+    if (static_cast<int64_t>(p.n_tokens) * c.n_heads > 0x3fffffff) {
+        MI_ERROR_FMT("mi_attention: %d rows of %d heads are more than a launch counts", p.n_tokens, c.n_heads);
+        return 0;
+    }
+    if (!ensure_init()) return 0;
+    AttentionArgs a{};
+    a.p = p;
+    a.q = static_cast<const uint16_t*>(c.q);
+    a.out = static_cast<uint16_t*>(c.out);
+    a.ld_q = c.ld_q;
+    a.ld_out = c.ld_out;
+    a.n_heads = c.n_heads;
+    a.kind = c.cache->kind;
+    a.head_dim = c.cache->head_dim;
+    a.max_tokens = c.batch->max_tokens;
+    a.window = c.window;
+    a.sinks = c.sinks;
+    a.scale = c.scale;
+    const auto s = static_cast<hipStream_t>(stream);
+    return launch_paged_attention(s, a, stream_workspace(s)) ? 1 : 0;
+}

@@ -137,6 +137,7 @@ WeightEntry weight_entry(const void* W) {
 uint64_t registry_epoch() { return g_registry_epoch.load(); }
 
 void* own_stream_workspace(hipStream_t s) { return s ? workspace_of(s) : nullptr; }
+void* stream_workspace(hipStream_t s) { return workspace_of(s); }
 
 StandsFor::StandsFor(hipStream_t recording, hipStream_t s) {
     t_recording = recording;
