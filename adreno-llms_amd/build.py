@@ -26,7 +26,7 @@ DEVICE = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-pa
 
 # (attention.hip takes every result of a matrix product through the vector units at once: with the
 #  accumulators in the general registers a key tile of its main loop loses 116 register moves)
-PER_SOURCE = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+PER_SOURCE = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("attention.hip", "paged_attention.hip")}
 
 
 def build(verbose=True, extra=()):
