@@ -21,9 +21,10 @@ bool paged_args(const char* who, const mi_kv_cache* cache, const mi_kv_batch* ba
 constexpr int row_bytes(int kind, int D) { return kind == MI_KV_F16 ? 2 * D : kind == MI_KV_INT8 ? D : D / 2; }
 constexpr int row_scales(int kind, int D) { return kind == MI_KV_F16 ? 0 : kind == MI_KV_INT8 ? 1 : D / 32; }
 
-// The number of row (page, head, slot), counted over all of a pool: at most 2^31 pages of fewer than 2^31 rows.
+// The number of row (page, head, slot), counted over all of a pool.  (A page has fewer than 2^31 rows: paged_args.)
 __device__ __forceinline__ int64_t row_number(const PagedArgs& a, int page, int head, int slot) {
-    return (static_cast<int64_t>(page) * a.n_kv_heads + head) * a.page.d + slot;
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(a.n_kv_heads * a.page.d)) +
+           static_cast<uint32_t>(head * a.page.d + slot);
 }
 
 // paged_attention.hip

@@ -9,6 +9,8 @@
 #include "device_math.h"
 #include "paged.h"
 
+#include <type_traits>
+
 namespace mi {
 namespace {
 
@@ -34,6 +36,12 @@ __device__ __forceinline__ float max_of_groups(float a) {
     r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// (fmaxf would quieten signalling NaNs first, an instruction for each operand)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{a, b}, half2v));
 }
@@ -49,10 +57,18 @@ __device__ __forceinline__ int scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // lane 31 to rows 2 and 3
     return x;
 }
-__device__ __forceinline__ float wave_sum(float x) {
-    #pragma unroll
-    for (int s = 32; s > 0; s /= 2) x += __shfl_xor(x, s);
-    return x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float add_dpp(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWS, 0xf, false));
+}
+// Sum of all lanes, in the last lane.
+__device__ __forceinline__ float sum_to_last(float x) {
+    x = add_dpp<0x111, 0xf>(x);
+    x = add_dpp<0x112, 0xf>(x);
+    x = add_dpp<0x114, 0xf>(x);
+    x = add_dpp<0x118, 0xf>(x);
+    x = add_dpp<0x142, 0xa>(x);
+    return add_dpp<0x143, 0xc>(x);
 }
 
 // ---- who does what --------------------------------------------------------------------------------------
@@ -70,7 +86,7 @@ struct Plan {                 // from the host
     Divider rep;              // by nrep
 };
 struct Item {
-    int b = -1, set = 0, chunk = 0, share = 0;
+    int b = -1, set = 0, chunk = 0, share = 0, tiles = 0;
     Span s;
 };
 
@@ -100,7 +116,8 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
             total += static_cast<float>(more.sets) * static_cast<float>(more.tiles);
         }
         // (a hundred-thousandth more: the sum's rounding must not make an item too many)
-        const float each = wave_sum(total) * 1.00001f / static_cast<float>(plan.target);
+        const float all = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_to_last(total)), 63));
+        const float each = all * 1.00001f / static_cast<float>(plan.target);
         it.share = each < 1.0e9f ? static_cast<int>(each) + 1 : 0x7fffffff;
         if (it.share < plan.least) it.share = plan.least;
         it.share = uniform(it.share);
@@ -115,10 +132,12 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
             it.s.first = __builtin_amdgcn_readlane(s.first, l);
             it.s.n = __builtin_amdgcn_readlane(s.n, l);
             it.s.pos = __builtin_amdgcn_readlane(s.pos, l);
+            it.tiles = __builtin_amdgcn_readlane(c.tiles, l);
             const int n = __builtin_amdgcn_readlane(chunks, l), sets = __builtin_amdgcn_readlane(c.sets, l);
             const int own = y - (__builtin_amdgcn_readlane(upto, l) - sets * n);
             it.set = sets == 1 ? 0 : own / n;
             it.chunk = own - it.set * n;
+            if (n > 1) it.share = (it.tiles - 1) / n + 1;          // (the sequence's tiles in n equal parts)
             return it;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
@@ -131,27 +150,32 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
 
 // ---- a tile of 32 keys as it comes from the cache, and as operands ------------------------------------------
 
-// Keys as A operand of q k: of 16 n + i, n = 0, 1, the elements g D / 4 .. (every group a quarter, so that pieces of rows are long;
-// which elements meet in one product does not matter as long as the query brings the same).  Values as A operand of
+// Keys as A operand of q k: of 16 n + i, n = 0, 1, pieces of 16 bytes (8 where a row has 32), the groups' side by side, so that
+// a load of 64 lanes covers 64 bytes and more of a row at once (with a quarter of the row per group every lane was in a line of its
+// own).  Which elements meet in one product does not matter as long as the query brings the same.  Values as A operand of
 // the product with the weights: of keys 4 g .. and 16 + 4 g .., the elements i D / 16 .., D / 16 of them, which become row i of
 // D / 16 operands: element m of the piece is row i of operand m.  The transpose is then one byte permute per two numbers.
-template <int KIND, int D>
+template <int KIND, int D, bool PAGES16>
 struct Tile {
-    static constexpr int kK = row_bytes(KIND, D) / 4 / 4;      // words of a key's piece
+    static constexpr int kK = row_bytes(KIND, D) / 4 / 4;      // words of a key's pieces
     static constexpr int kVBytes = row_bytes(KIND, D) / 16;    // bytes of a value's piece: 2, 4, 8, 16
     static constexpr int kV = (kVBytes + 3) / 4;
-    uint32_t k[2][kK], v[8][kV];
-    uint16_t ks[2], vs[8];                                     // their scales
-    bool bad[2];                                               // 16 keys whose page is not in the pool (pages by 16 keys)
-    uint32_t absent;                                           // bit e: key e of the lane's values, bit 8 + n: its key n has no page
+    uint32_t k[2][kK];
+    std::conditional_t<kVBytes == 2, uint16_t, uint32_t> v[8][kV];
+    uint16_t ks[2];                                            // the keys' scales
+    // The values' scales, of four keys at a time as they are loaded: Q4 whole rows of them; int8 two to a word, or (keys looked up
+    // one by one) one to a word.  pack_scales leaves the lane's, two to a word, in the first two.
+    static constexpr int kVS = KIND == MI_KV_Q4 ? D / 16 : PAGES16 ? 2 : 4;
+    uint32_t vs[2][kVS];
 };
 
-template <int N>
+// N words, in pieces of four that are 4 STEP bytes apart.
+template <int STEP, int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
     if constexpr (N % 4 == 0) {
         #pragma unroll
         for (int j = 0; j < N; j += 4) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(p + 4 * j);
+            const u32x4 x = *reinterpret_cast<const u32x4*>(p + STEP * j);
             w[j] = x[0]; w[j + 1] = x[1]; w[j + 2] = x[2]; w[j + 3] = x[3];
         }
     } else if constexpr (N == 2) {
@@ -162,68 +186,113 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* p) {
     }
 }
 
-// Codes as fp16 numbers: a byte (plus 128) or nibble (plus 8) under the exponent of 1024 is that number above 1024.
-__device__ __forceinline__ uint32_t from_codes(uint32_t w, _Float16 above, half2v scale) {
-    const half2v x = (__builtin_bit_cast(half2v, w) - half2v{above, above}) * scale;
-    return __builtin_bit_cast(uint32_t, x);
+template <int N>
+__device__ __forceinline__ void load_value(uint32_t (&w)[N], const uint8_t* p) { load_words<4>(w, p); }
+__device__ __forceinline__ void load_value(uint16_t (&w)[1], const uint8_t* p) { w[0] = *reinterpret_cast<const uint16_t*>(p); }
+
+// Codes as fp16 numbers, two to a word, times their scales: rounded once, to the number that the cache holds.
+__device__ __forceinline__ uint32_t scaled(uint32_t codes, half2v scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, codes) * scale);
+}
+// Signed bytes LO of a and HI of b.  (Sub-word operands: an instruction per number, where building it under an exponent takes three
+// for two.)
+template <int LO, int HI>
+__device__ __forceinline__ uint32_t from_bytes(uint32_t a, uint32_t b) {
+    uint32_t r;
+#define MI_BYTES(L, H)                                                                                                     \
+    if constexpr (LO == L && HI == H)                                                                                      \
+        asm("v_cvt_f16_i16_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_" #L "\n\t"                 \
+            "v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_" #H                  \
+            : "=&v"(r) : "v"(a), "v"(b))
+    MI_BYTES(0, 0);
+    MI_BYTES(1, 1);
+    MI_BYTES(2, 2);
+    MI_BYTES(3, 3);
+    MI_BYTES(0, 1);
+    MI_BYTES(2, 3);
+#undef MI_BYTES
+    return r;
+}
+// The nibbles at bits 0 and 16, less 8: under the exponent of 1024 a nibble is that number above 1024.  (Both constants cannot
+// be scalars of one instruction: `exponent` is a vector register that holds 0x64006400.)
+__device__ __forceinline__ uint32_t from_nibbles(uint32_t w, uint32_t exponent) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(0x000f000fu), "v"(exponent));
+    const half2v above = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, r) - above);
 }
 __device__ __forceinline__ half2v both(uint16_t s) { return __builtin_bit_cast(half2v, s * 0x00010001u); }
 
 // Operand j (8 elements) of a key's piece.  Q4: elements come as 0 4 1 5 2 6 3 7 of each 8, and so does the query.
 template <int KIND, int N>
-__device__ __forceinline__ half8 key_operand(const uint32_t (&w)[N], int j, uint16_t scale) {
+__device__ __forceinline__ half8 key_operand(const uint32_t (&w)[N], int j, uint16_t scale, uint32_t exponent) {
     if constexpr (KIND == MI_KV_F16) return __builtin_bit_cast(half8, u32x4{w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]});
     u32x4 r;
     const half2v s = both(scale);
     if constexpr (KIND == MI_KV_INT8) {
         #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t u = w[2 * j + h];
-            r[2 * h] = from_codes(__builtin_amdgcn_perm(0, u, 0x0c010c00u) ^ 0x64806480u, static_cast<_Float16>(1152.0f), s);
-            r[2 * h + 1] = from_codes(__builtin_amdgcn_perm(0, u, 0x0c030c02u) ^ 0x64806480u, static_cast<_Float16>(1152.0f), s);
+            r[2 * h] = scaled(from_bytes<0, 1>(w[2 * j + h], w[2 * j + h]), s);
+            r[2 * h + 1] = scaled(from_bytes<2, 3>(w[2 * j + h], w[2 * j + h]), s);
         }
     } else {
         #pragma unroll
-        for (int h = 0; h < 4; ++h)
-            r[h] = from_codes(((w[j] >> (4 * h)) & 0x000f000fu) | 0x64006400u, static_cast<_Float16>(1032.0f), s);
+        for (int h = 0; h < 4; ++h) r[h] = scaled(from_nibbles(w[j] >> (4 * h), exponent), s);
     }
     return __builtin_bit_cast(half8, r);
 }
 
+// (Lane i's elements i D / 16 .. of a Q4 row are in block i D / 16 / 32 of it.)
+template <int KIND, int D, bool PAGES16>
+__device__ __forceinline__ void pack_scales(Tile<KIND, D, PAGES16>& t, int i) {
+    if constexpr (KIND == MI_KV_F16 || (KIND == MI_KV_INT8 && PAGES16)) return;
+    constexpr int kWords = KIND == MI_KV_Q4 ? D / 64 : 1;          // of a key
+    const uint32_t sel = KIND == MI_KV_Q4 && i & (8 / kWords) ? 0x07060302u : 0x05040100u;
+    #pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        uint32_t w[4];
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = kWords == 1 || i < 8 ? t.vs[n][kWords * e] : t.vs[n][kWords * e + kWords - 1];
+        t.vs[n][0] = __builtin_amdgcn_perm(w[1], w[0], sel);
+        t.vs[n][1] = __builtin_amdgcn_perm(w[3], w[2], sel);
+    }
+}
+
 // Keys 2 p and 2 p + 1 of the lane's values, element m of their pieces.
-template <int KIND, int D>
-__device__ __forceinline__ uint32_t value_pair(const Tile<KIND, D>& t, int p, int m) {
+template <int KIND, int D, bool PAGES16>
+__device__ __forceinline__ uint32_t value_pair(const Tile<KIND, D, PAGES16>& t, int p, int m, uint32_t exponent) {
     const auto &lo = t.v[2 * p], &hi = t.v[2 * p + 1];
     if constexpr (KIND == MI_KV_F16)
         return __builtin_amdgcn_perm(hi[m / 2], lo[m / 2], m & 1 ? 0x07060302u : 0x05040100u);
-    const half2v s = __builtin_bit_cast(half2v, static_cast<uint32_t>(t.vs[2 * p]) | static_cast<uint32_t>(t.vs[2 * p + 1]) << 16);
+    const half2v s = __builtin_bit_cast(half2v, t.vs[p / 2][p % 2]);
     if constexpr (KIND == MI_KV_INT8) {
-        const uint32_t sel = 0x0c040c00u + 0x00010001u * (m % 4);
-        return from_codes(__builtin_amdgcn_perm(hi[m / 4], lo[m / 4], sel) ^ 0x64806480u, static_cast<_Float16>(1152.0f), s);
+        const uint32_t a = lo[m / 4], b = hi[m / 4];
+        return scaled(m % 4 == 0 ? from_bytes<0, 0>(a, b) : m % 4 == 1 ? from_bytes<1, 1>(a, b) : m % 4 == 2 ? from_bytes<2, 2>(a, b)
+                                                                                                           : from_bytes<3, 3>(a, b), s);
     } else {
-        const uint32_t two = __builtin_amdgcn_perm(hi[0], lo[0], m < 4 ? 0x05040100u : 0x07060302u);
-        return from_codes(((two >> (4 * (m % 4))) & 0x000f000fu) | 0x64006400u, static_cast<_Float16>(1032.0f), s);
+        const uint32_t two = __builtin_amdgcn_perm(static_cast<uint32_t>(hi[0]), static_cast<uint32_t>(lo[0]), m < 4 ? 0x05040100u : 0x07060302u);
+        return scaled(from_nibbles(two >> (4 * (m % 4)), exponent), s);
     }
 }
 
 // Whether any of the lane's values that are in the cache (`there`, a mask for each pair of keys) may be an infinity or a NaN:
 // of fp16 its greatest, else its scales (256 and more count, as their products may overflow).
-template <int KIND, int D>
-__device__ __forceinline__ bool odd_values(const Tile<KIND, D>& t, const uint32_t (&there)[4]) {
+template <int KIND, int D, bool PAGES16>
+__device__ __forceinline__ bool odd_values(const Tile<KIND, D, PAGES16>& t, const uint32_t (&there)[4]) {
     uint16_t most = 0;
     #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const uint16_t have = static_cast<uint16_t>(there[e / 2] >> (16 * (e & 1)));
         if constexpr (KIND == MI_KV_F16) {
             #pragma unroll
-            for (int w = 0; w < Tile<KIND, D>::kV; ++w)
+            for (int w = 0; w < Tile<KIND, D, PAGES16>::kV; ++w)
                 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint16_t x = static_cast<uint16_t>(t.v[e][w] >> (16 * h)) & have & 0x7fffu;
                     most = x > most ? x : most;
                 }
         } else {
-            const uint16_t x = t.vs[e] & have & 0x7fffu;
+            const uint16_t x = static_cast<uint16_t>(t.vs[e / 4][e / 2 % 2] >> (16 * (e & 1))) & have & 0x7fffu;
             most = x > most ? x : most;
         }
     }
@@ -233,15 +302,16 @@ __device__ __forceinline__ bool odd_values(const Tile<KIND, D>& t, const uint32_
 // ---- few rows: keys straight from memory to registers -----------------------------------------------------
 
 constexpr int kRows = 16, kKeys = 32;
-constexpr int kWaves = 4;                          // wavefronts per block; they take the block's tiles in turn
+constexpr int kWaves = 4;                     // wavefronts per block; they take the block's tiles in turn
 constexpr int slot_floats(int D) { return 16 * D + 32; }
 
 // PAGES16: pages are multiples of 16 positions long, so 16 keys lie in one page.
 template <int KIND, int D, bool PAGES16>
-__global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ sums,
+__global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ sums,
                                                                  uint32_t* __restrict__ counters) {
     constexpr int kOps = D / 32, kOuts = D / 16;   // operands of a key, of the values
     constexpr int kRow = row_bytes(KIND, D), kScales = row_scales(KIND, D);
+    constexpr int kPiece = kRow >= 64 ? 16 : 8, kElems = kPiece * D / kRow;       // of a key: bytes, elements
     __shared__ float meet[kWaves][4 * kOuts + 2][64];
     __shared__ uint32_t arrived;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -260,74 +330,104 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
     const bool live = r0 + i < r_end;
     const int row = live ? r0 + i : r_end - 1, token = divide(row, plan.rep), head = kvh * plan.nrep + (row - token * plan.nrep);
     const int my_pos = it.s.pos + token;
+    // (a row before position 0 sees nothing; the window's far end, before the first position where there is none)
+    const int before = (a.window > 0 && my_pos >= 0) ? my_pos - a.window : -1, sinks = a.window > 0 ? a.sinks : 0;
     half8 q[kOps];
     {
-        const uint16_t* src = a.q + (it.s.first + token) * a.ld_q + head * D + g * (D / 4);
+        const uint16_t* src = a.q + (it.s.first + token) * a.ld_q + head * D + g * kElems;
         const bool wide = reinterpret_cast<uintptr_t>(src) % 16 == 0;
         #pragma unroll
         for (int j = 0; j < kOps; ++j) {
+            constexpr int kPer = kElems / 8;           // operands of a piece
+            const uint16_t* at = src + j / kPer * (4 * kElems) + 8 * (j % kPer);
             half8 x;
-            if (wide) x = *reinterpret_cast<const half8*>(src + 8 * j);
+            if (wide) x = *reinterpret_cast<const half8*>(at);
             else
                 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(_Float16, src[8 * j + e]);
+                for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(_Float16, at[e]);
             q[j] = KIND == MI_KV_Q4 ? __builtin_shufflevector(x, x, 0, 4, 1, 5, 2, 6, 3, 7) : x;
         }
     }
 
-    const int* const table = a.p.pages + static_cast<int64_t>(it.b) * a.p.max_pages;
-    auto fetch = [&](Tile<KIND, D>& t, int v) {
-        const int j0 = tile_at(tiles, v) * kKeys;
-        t.absent = 0;
-        t.bad[0] = t.bad[1] = false;
+    // (as constant memory: scalar loads where the page is one for the wavefront, which do not wait for the tile under way)
+    const auto* const table = reinterpret_cast<const __attribute__((address_space(4))) int*>(
+        reinterpret_cast<uintptr_t>(a.p.pages + static_cast<int64_t>(it.b) * a.p.max_pages));
+    // Page numbers are asked for a tile ahead of what lies in them: two loads in a row would be waited for otherwise.
+    struct Pages { int number[2]; };
+    auto look_up = [&](int v) {
+        Pages p;
+        const int j0 = tile_at(tiles, v < last ? v : last - 1) * kKeys;
         #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const uint8_t *kp, *vp[4];
-            const uint16_t *ksp = nullptr, *vsp[4] = {};
+            const int mine = j0 + 16 * n + (PAGES16 ? 0 : i), j = mine < tiles.end ? mine : tiles.end - 1;
+            p.number[n] = table[divide(j, a.p.page)];
+        }
+        return p;
+    };
+    // A load's address is a base that is the same for the wavefront plus 32 bits of the lane's own.
+    const uint32_t k_off = i * kRow + g * kPiece, v_off = 4 * g * kRow + i * (kRow / 16);
+    const uint32_t ks_off = (i * kScales + kScales * g / 4) * 2, vs_off = 4 * g * kScales * 2;
+    struct Rows {                                  // of a tile: where its two times 16 rows begin, and what is not in the pool:
+        int64_t at[2];                             // (PAGES16: of 16 keys; else of the lane's key)
+        uint32_t absent;                           // bit e of 8: key e of the lane's values
+    };
+    auto place = [&](int v, const Pages& pages) {
+        Rows r;
+        r.absent = 0;
+        const int j0 = tile_at(tiles, v) * kKeys;
+        #pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int mine = j0 + 16 * n + (PAGES16 ? 0 : i), j = mine < tiles.end ? mine : tiles.end - 1;
+            const int number = pages.number[n];
+            const bool bad = static_cast<uint32_t>(number) >= static_cast<uint32_t>(a.p.n_pages);
+            int slot = j - divide(j, a.p.page) * a.p.page.d;
+            // (16 keys behind the end are read as the last 16 before it, and masked)
+            if constexpr (PAGES16) slot &= ~15;
+            r.at[n] = row_number(a.p, bad ? 0 : number, kvh, slot);
             if constexpr (PAGES16) {
-                const int j = j0 + 16 * n < tiles.end ? j0 + 16 * n : j0;
-                const int page = divide(j, a.p.page);
-                int number = uniform(table[page]);
-                t.bad[n] = number < 0 || number >= a.p.n_pages;
-                number = t.bad[n] ? 0 : number;
-                const int64_t at = row_number(a.p, number, kvh, j - page * a.p.page.d);
-                kp = a.p.k + at * kRow + i * kRow + g * (kRow / 4);
-                const uint8_t* vb = a.p.v + at * kRow + 4 * g * kRow + i * (kRow / 16);
-                #pragma unroll
-                for (int e = 0; e < 4; ++e) vp[e] = vb + e * kRow;
-                if constexpr (kScales > 0) {
-                    ksp = a.p.k_scale + at * kScales + i * kScales;
-                    const uint16_t* vsb = a.p.v_scale + at * kScales + 4 * g * kScales;
-                    #pragma unroll
-                    for (int e = 0; e < 4; ++e) vsp[e] = vsb + e * kScales;
-                }
+                if (bad) r.absent |= 15u << (4 * n);
             } else {
-                const int mine = j0 + 16 * n + i, j = mine < tiles.end ? mine : tiles.end - 1;
-                const int page = divide(j, a.p.page), number = table[page];
-                const bool none = number < 0 || number >= a.p.n_pages;
-                if (none) t.absent |= 256u << n;
-                const int64_t at = row_number(a.p, none ? 0 : number, kvh, j - page * a.p.page.d);
-                kp = a.p.k + at * kRow + g * (kRow / 4);
-                ksp = a.p.k_scale + at * kScales;
-                const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
                 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int64_t from = static_cast<uint32_t>(__shfl(at_lo, 4 * g + e)) | static_cast<int64_t>(__shfl(at_hi, 4 * g + e)) << 32;
-                    if (__shfl(static_cast<int>(none), 4 * g + e)) t.absent |= 1u << (4 * n + e);
-                    vp[e] = a.p.v + from * kRow + i * (kRow / 16);
-                    vsp[e] = a.p.v_scale + from * kScales;
-                }
+                for (int e = 0; e < 4; ++e) r.absent |= __shfl(bad ? 1u << (4 * n + e) : 0u, 4 * g + e);
             }
-            load_words(t.k[n], kp);
+        }
+        return r;
+    };
+    Tile<KIND, D, PAGES16> t;
+    uint32_t exponent = 0x64006400u;               // see from_nibbles
+    if constexpr (KIND == MI_KV_Q4) asm("" : "+v"(exponent));
+    auto load_keys = [&](const Rows& r) {
+        #pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            if constexpr (PAGES16) {
+                load_words<16>(t.k[n], a.p.k + r.at[n] * kRow + k_off);
+                if constexpr (kScales > 0)
+                    t.ks[n] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.p.k_scale + r.at[n] * kScales) + ks_off);
+            } else {
+                load_words<16>(t.k[n], a.p.k + r.at[n] * kRow + g * kPiece);
+                if constexpr (kScales > 0) t.ks[n] = a.p.k_scale[r.at[n] * kScales + kScales * g / 4];
+            }
+        }
+    };
+    auto load_values = [&](const Rows& r) {
+        #pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            if constexpr (PAGES16 && kScales > 0)
+                load_words<4>(t.vs[n], reinterpret_cast<const uint8_t*>(a.p.v_scale + r.at[n] * kScales) + vs_off);
             #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                if constexpr (Tile<KIND, D>::kVBytes == 2) t.v[4 * n + e][0] = *reinterpret_cast<const uint16_t*>(vp[e]);
-                else load_words(t.v[4 * n + e], vp[e]);
-            }
-            if constexpr (kScales > 0) {
-                t.ks[n] = ksp[kScales * g / 4];
-                #pragma unroll
-                for (int e = 0; e < 4; ++e) t.vs[4 * n + e] = vsp[e][kScales * i / 16];
+                if constexpr (PAGES16) {
+                    load_value(t.v[4 * n + e], a.p.v + r.at[n] * kRow + v_off + e * kRow);
+                } else {
+                    const int lo = static_cast<int>(r.at[n]), hi = static_cast<int>(r.at[n] >> 32);
+                    const int64_t from = static_cast<uint32_t>(__shfl(lo, 4 * g + e)) | static_cast<int64_t>(__shfl(hi, 4 * g + e)) << 32;
+                    load_value(t.v[4 * n + e], a.p.v + from * kRow + i * (kRow / 16));
+                    if constexpr (KIND == MI_KV_INT8) t.vs[n][e] = a.p.v_scale[from];
+                    if constexpr (KIND == MI_KV_Q4)
+                        #pragma unroll
+                        for (int w = 0; w < D / 64; ++w)
+                            t.vs[n][e * (D / 64) + w] = reinterpret_cast<const uint32_t*>(a.p.v_scale + from * kScales)[w];
+                }
             }
         }
     };
@@ -342,7 +442,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
     for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
     const float scale_log2 = a.scale * 1.44269504088896341f;
 
-    auto multiply = [&](const Tile<KIND, D>& t, int v) {
+    // Tile v, whose rows are `r`; `more`: the keys and values of tile v + kWaves, at `next`, are asked for as soon as the registers of
+    // tile v's are free, so that they are on their way meanwhile without registers of their own.
+    auto multiply = [&](int v, const Rows& r, auto more, const Rows& next) {
         const int j0 = tile_at(tiles, v) * kKeys;
         floatx4 s[2];
         #pragma unroll
@@ -350,27 +452,25 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
             s[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             #pragma unroll
             for (int j = 0; j < kOps; ++j)
-                s[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_operand<KIND>(t.k[n], j, t.ks[n]), q[j], s[n], 0, 0, 0);
+                s[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key_operand<KIND>(t.k[n], j, t.ks[n], exponent), q[j], s[n], 0, 0, 0);
         }
+        if constexpr (more.value) load_keys(next);
         bool masked = !all_seen(j0, kKeys, p_lo, p_hi, a.p.cap, a.window, a.sinks);
-        if constexpr (PAGES16) masked |= t.bad[0] || t.bad[1];
-        else masked |= __any(t.absent);
-        uint32_t there[4];                         // halves of keys that are in the cache at all
+        masked |= PAGES16 ? r.absent != 0 : __any(r.absent);
+        uint32_t there[4] = {};                    // halves of keys that are in the cache at all
         if (masked) {
+            asm volatile("");                      // (a branch: most tiles are not)
             #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = j0 + 16 * n + 4 * g + r, e = 4 * n + r;
-                    const bool have = j < tiles.end && !(PAGES16 ? t.bad[n] : (t.absent >> e & 1) != 0);
-                    if (!have || !sees(my_pos, j, a.window, a.sinks)) s[n][r] = kNone;
-                    const uint32_t half = have ? 0xffffu << (16 * (e & 1)) : 0u;
-                    there[e / 2] = e & 1 ? there[e / 2] | half : half;
-                }
+            for (int e = 0; e < 8; ++e) {
+                const int n = e / 4, j = j0 + 16 * n + 4 * g + e % 4;
+                const bool have = (j < tiles.end) & ((r.absent >> e & 1) == 0);
+                const bool see = have & (j <= my_pos) & ((j > before) | (j < sinks));
+                s[n][e % 4] = see ? s[n][e % 4] : kNone;
+                there[e / 2] |= have ? 0xffffu << (16 * (e & 1)) : 0u;
             }
         }
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = top * scale_log2 - kHead;
+        float top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max3(s[1][2], s[1][3], s[1][3]));
+        top = fmaf(top, scale_log2, -kHead);
         if (__any(top > base + kSlack)) {
             top = fmaxf(base, max_of_groups(top));
             const float alpha = __builtin_amdgcn_exp2f(base - top);
@@ -382,14 +482,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
         float w[8];
         #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], scale_log2, -base));
+        pack_scales(t, i);
         const half8 pb = __builtin_bit_cast(half8, u32x4{pack2(w[0], w[1]), pack2(w[2], w[3]), pack2(w[4], w[5]), pack2(w[6], w[7])});
         l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb, l, 0, 0, 0);
         if (!masked) {
             #pragma unroll
             for (int m = 0; m < kOuts; ++m)
                 acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                    __builtin_bit_cast(half8, u32x4{value_pair(t, 0, m), value_pair(t, 1, m), value_pair(t, 2, m), value_pair(t, 3, m)}),
+                    __builtin_bit_cast(half8, u32x4{value_pair(t, 0, m, exponent), value_pair(t, 1, m, exponent), value_pair(t, 2, m, exponent), value_pair(t, 3, m, exponent)}),
                     pb, acc[m], 0, 0, 0);
+            if constexpr (more.value) load_values(next);
             return;
         }
         // A masked key has weight 0, but 0 x inf and 0 x NaN are NaN.  What is not in the cache is taken as 0; where there is
@@ -398,12 +500,13 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
         auto product = [&](int m, const uint32_t (&mask)[4]) {
             u32x4 x;
             #pragma unroll
-            for (int p = 0; p < 4; ++p) x[p] = value_pair(t, p, m) & mask[p];
+            for (int p = 0; p < 4; ++p) x[p] = value_pair(t, p, m, exponent) & mask[p];
             return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, x), pb, acc[m], 0, 0, 0);
         };
         if (!__any(odd_values(t, there))) {
             #pragma unroll
             for (int m = 0; m < kOuts; ++m) acc[m] = product(m, there);
+            if constexpr (more.value) load_values(next);
             return;
         }
         #pragma unroll 1
@@ -422,27 +525,29 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
                 if (i == z) acc[m] = mine;
             }
         }
+        if constexpr (more.value) load_values(next);
     };
 
-    // One tile on its way while the one before it is multiplied (past the last: that one again, from the cache).
     if (first + wave < last) {
-        Tile<KIND, D> x, z;
         int v = first + wave;
-        fetch(x, v);
-        for (;;) {
-            fetch(z, v + kWaves < last ? v + kWaves : v);
-            multiply(x, v);
-            v += kWaves;
-            if (v >= last) break;
-            fetch(x, v + kWaves < last ? v + kWaves : v);
-            multiply(z, v);
-            v += kWaves;
-            if (v >= last) break;
+        Pages pages = look_up(v);
+        Rows now = place(v, pages);
+        load_keys(now);
+        load_values(now);
+        pages = look_up(v + kWaves);
+        for (; v + kWaves < last; v += kWaves) {
+            const Rows next = place(v + kWaves, pages);
+            pages = look_up(v + 2 * kWaves);
+            multiply(v, now, std::true_type{}, next);
+            now = next;
         }
+        multiply(v, now, std::false_type{}, now);
     }
 
-    // The wavefronts' sums meet in LDS; wavefront w goes on with register w of every output, that is with elements
-    // (4 g + w) D / 16 .. of query i.
+    // The wavefronts' sums meet in LDS; wavefront w goes on with register w % 4 of some outputs, that is with kMine elements from
+    // `element` on of query i.
+    constexpr int kMine = kOuts * 4 / kWaves;
+    const int reg = wave % 4, m0 = wave / 4 * kMine, element = (4 * g + reg) * kOuts + m0;
     float* const mine = &meet[wave][0][lane];
     mine[0] = base;
     mine[64] = l[0];
@@ -454,15 +559,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
     float top = meet[0][0][lane];
     #pragma unroll
     for (int z = 1; z < kWaves; ++z) top = fmaxf(top, meet[z][0][lane]);
-    float sum = 0.0f, o[kOuts];
+    float sum = 0.0f, o[kMine];
     #pragma unroll
-    for (int m = 0; m < kOuts; ++m) o[m] = 0.0f;
+    for (int m = 0; m < kMine; ++m) o[m] = 0.0f;
     #pragma unroll
     for (int z = 0; z < kWaves; ++z) {
         const float f = __builtin_amdgcn_exp2f(meet[z][0][lane] - top);
         sum += meet[z][1][lane] * f;
         #pragma unroll
-        for (int m = 0; m < kOuts; ++m) o[m] += meet[z][2 + m * 4 + wave][lane] * f;
+        for (int m = 0; m < kMine; ++m) o[m] += meet[z][2 + (m0 + m) * 4 + reg][lane] * f;
     }
 
     if (parts > 1) {
@@ -472,11 +577,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
         auto* const slot = reinterpret_cast<uint64_t*>(sums) + static_cast<int64_t>(blockIdx.x) * kSlot;
         if (live) {
             #pragma unroll
-            for (int m = 0; m < kOuts; m += 2)
-                __hip_atomic_store(slot + m / 2 * 256 + tid, __builtin_bit_cast(uint64_t, floatx2{o[m], o[m + 1]}), __ATOMIC_RELAXED,
+            for (int m = 0; m < kMine; m += 2)
+                __hip_atomic_store(slot + m / 2 * (64 * kWaves) + tid, __builtin_bit_cast(uint64_t, floatx2{o[m], o[m + 1]}), __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
             if (wave == 0 && g == 0)
-                __hip_atomic_store(slot + kOuts / 2 * 256 + i, __builtin_bit_cast(uint64_t, floatx2{top, sum}), __ATOMIC_RELAXED,
+                __hip_atomic_store(slot + 8 * D + i, __builtin_bit_cast(uint64_t, floatx2{top, sum}), __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -495,37 +600,44 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void paged_step_kern
             return __builtin_bit_cast(floatx2, __hip_atomic_load(slots + part * next + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         };
         top = kStart;
-        #pragma unroll 4
-        for (int z = 0; z < parts; ++z) top = fmaxf(top, pair_at(z, kOuts / 2 * 256 + col)[0]);
         sum = 0.0f;
         #pragma unroll
-        for (int m = 0; m < kOuts; ++m) o[m] = 0.0f;
+        for (int m = 0; m < kMine; ++m) o[m] = 0.0f;
         const int at = live ? tid : tid & ~15;
-        #pragma unroll 4
-        for (int z = 0; z < parts; ++z) {
-            const floatx2 bl = pair_at(z, kOuts / 2 * 256 + col);
-            const float f = __builtin_amdgcn_exp2f(bl[0] - top);
-            sum += bl[1] * f;
+        constexpr int kAhead = 32 / kMine;                     // parts asked for together
+        for (int z0 = 0; z0 < parts; z0 += kAhead) {
+            floatx2 bl[kAhead], x[kAhead][kMine / 2];
             #pragma unroll
-            for (int m = 0; m < kOuts; m += 2) {
-                const floatx2 x = pair_at(z, m / 2 * 256 + at);
-                o[m] += x[0] * f;
-                o[m + 1] += x[1] * f;
+            for (int z = 0; z < kAhead; ++z) {
+                const int part = z0 + z < parts ? z0 + z : parts - 1;
+                bl[z] = pair_at(part, 8 * D + col);
+                #pragma unroll
+                for (int m = 0; m < kMine; m += 2) x[z][m / 2] = pair_at(part, m / 2 * (64 * kWaves) + at);
+            }
+            #pragma unroll
+            for (int z = 0; z < kAhead; ++z) {
+                if (z0 + z >= parts) break;
+                const float now = fmaxf(top, bl[z][0]), was = __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(bl[z][0] - now);
+                top = now;
+                sum = sum * was + bl[z][1] * f;
+                #pragma unroll
+                for (int m = 0; m < kMine; ++m) o[m] = o[m] * was + x[z][m / 2][m & 1] * f;
             }
         }
     }
     if (!live) return;
     const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
-    uint16_t* const dst = a.out + (it.s.first + token) * a.ld_out + head * D + (4 * g + wave) * kOuts;
-    uint32_t h[kOuts / 2];
+    uint16_t* const dst = a.out + (it.s.first + token) * a.ld_out + head * D + element;
+    uint32_t h[kMine / 2];
     #pragma unroll
-    for (int m = 0; m < kOuts; m += 2) h[m / 2] = pack2(o[m] * inv, o[m + 1] * inv);
-    if (reinterpret_cast<uintptr_t>(dst) % (2 * kOuts) == 0) {
-        if constexpr (kOuts == 8) *reinterpret_cast<u32x4*>(dst) = u32x4{h[0], h[1], h[2], h[3]};
-        else *reinterpret_cast<u32x2*>(dst) = u32x2{h[0], h[1]};
+    for (int m = 0; m < kMine; m += 2) h[m / 2] = pack2(o[m] * inv, o[m + 1] * inv);
+    if (reinterpret_cast<uintptr_t>(dst) % (2 * kMine) == 0) {
+        if constexpr (kMine == 8) *reinterpret_cast<u32x4*>(dst) = u32x4{h[0], h[1], h[2], h[3]};
+        else if constexpr (kMine == 4) *reinterpret_cast<u32x2*>(dst) = u32x2{h[0], h[1]};
+        else *reinterpret_cast<uint32_t*>(dst) = h[0];
     } else {
         #pragma unroll
-        for (int m = 0; m < kOuts; ++m) dst[m] = static_cast<uint16_t>(h[m / 2] >> (16 * (m & 1)));
+        for (int m = 0; m < kMine; ++m) dst[m] = static_cast<uint16_t>(h[m / 2] >> (16 * (m & 1)));
     }
 }
 
@@ -534,14 +646,14 @@ bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace) {
     Plan plan{};
     plan.nrep = a.n_heads / a.p.n_kv_heads;
     plan.rep = make_divider(plan.nrep);
-    plan.least = 8;
+    plan.least = 16;
     // Sets of 16 rows: at most one more per sequence than full ones.
     const int64_t rows = static_cast<int64_t>(a.p.n_tokens) * plan.nrep, seqs = a.p.n_seqs < a.p.n_tokens ? a.p.n_seqs : a.p.n_tokens;
     const int64_t sets = (rows - seqs) / kRows + seqs;
     // Items beside one per set: as many blocks as the chip holds.
     const int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (slot_floats(D) * sizeof(float))) : 0;
     int64_t blocks = sets * a.p.n_kv_heads;
-    const int64_t want = 4 * device_info().cus, room = (slots < kSliceCounters ? slots : kSliceCounters) - blocks;
+    const int64_t want = 3 * device_info().cus, room = (slots < kSliceCounters ? slots : kSliceCounters) - blocks;
     const int64_t target = (want < room ? want : room) / a.p.n_kv_heads;
     plan.target = target > 0 ? static_cast<int>(target) : 0;
     blocks += static_cast<int64_t>(plan.target) * a.p.n_kv_heads;
