@@ -18,6 +18,8 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short short4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -73,7 +75,7 @@ __device__ __forceinline__ float sum_to_last(float x) {
 
 // ---- who does what --------------------------------------------------------------------------------------
 //
-// The lengths are known to the device alone.  A block works on some tiles of keys for 16 ROWS-row sets of one sequence and
+// The lengths are known to the device alone.  A block works on some tiles of keys for a set of ROWS rows of one sequence and
 // key/value head; how many tiles that are follows from the tiles of the whole batch, so that every block gets about as
 // many whatever the mixture of lengths: `share` tiles, such that the items fit the `target` blocks that the chip holds plus
 // one per set.  Every wavefront works that out for itself from q_start and kv_len: the loads are those that it
@@ -82,6 +84,7 @@ __device__ __forceinline__ float sum_to_last(float x) {
 struct Plan {                 // from the host
     int target;               // items per key/value head beside one per set; 0: keys are not split
     int least;                // tiles of keys that a block is worth
+    int from, to;             // sequences of that many rows (new tokens times nrep) are the launch's
     int nrep;
     Divider rep;              // by nrep
 };
@@ -93,7 +96,7 @@ struct Item {
 struct Cost { int sets, tiles; };
 template <int ROWS, int KEYS>
 __device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Plan& plan, const Span& s) {
-    if (s.n <= 0) return {0, 0};
+    if (s.n <= 0 || s.n * plan.nrep < plan.from || s.n * plan.nrep > plan.to) return {0, 0};
     const int count = tiles_of(s.pos, s.pos + s.n - 1, a.p.cap, a.window, a.sinks, KEYS).count;
     return {(s.n * plan.nrep + ROWS - 1) / ROWS, count > 0 ? count : 1};
 }
@@ -135,8 +138,9 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
             it.tiles = __builtin_amdgcn_readlane(c.tiles, l);
             const int n = __builtin_amdgcn_readlane(chunks, l), sets = __builtin_amdgcn_readlane(c.sets, l);
             const int own = y - (__builtin_amdgcn_readlane(upto, l) - sets * n);
-            it.set = sets == 1 ? 0 : own / n;
-            it.chunk = own - it.set * n;
+            const int set = sets == 1 ? 0 : own / n;
+            it.chunk = own - set * n;
+            it.set = sets - 1 - set;                                 // (the longest first)
             if (n > 1) it.share = (it.tiles - 1) / n + 1;          // (the sequence's tiles in n equal parts)
             return it;
         }
@@ -641,38 +645,433 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kern
     }
 }
 
-template <int KIND, int D>
-bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace) {
+// ---- many rows: tiles of keys in LDS, 32 rows per wavefront -------------------------------------------------
+//
+// A block has 128 rows of one sequence and key/value head, 32 per wavefront (v_mfma_f32_32x32x16_f16: twice the rows per
+// operand that comes out of LDS), and takes its tiles of 64 keys through two buffers in LDS: while a tile is multiplied the next one
+// is on its way to registers, and is written (int8 and Q4: as fp16, converted once for the block) behind it.
+// Scores again transposed: lane (query = lane % 32, half h = lane / 32) has keys 8 a + 4 h + b of every 32, a, b = 0 .. 3, in
+// registers 4 a + b, and registers 8 c .. 8 c + 7 are the B operand of the product with the values for keys 16 c + 4 h .. and 16 c + 8 +
+// 4 h ..  The A operand, 4 keys of one element at a time, is what a transposed read from LDS gives.
+// In a row of LDS the 16-byte piece p lies at p ^ twist(row): eight rows' pieces of one p, and four rows' two neighbouring pieces,
+// are in different banks.
+
+constexpr int kChunkKeys = 64, kChunkWaves = 4, kChunkRows = 32 * kChunkWaves;
+constexpr int chunk_slot_floats(int D) { return kChunkRows * (D + 2); }
+constexpr int chunk_lds(int D) { return 2 * 2 * kChunkKeys * 2 * D; }
+__device__ __forceinline__ constexpr int twist(int row) { return (row & 3) * 2 + (row >> 2 & 1); }
+
+template <int KIND, int D, bool PAGES16>
+__global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ sums,
+                                                                          uint32_t* __restrict__ counters) {
+    constexpr int kRow = row_bytes(KIND, D), kScales = row_scales(KIND, D);
+    constexpr int kPiece = KIND == MI_KV_Q4 && D == 64 ? 8 : 16, kPieces = kRow / kPiece;      // of a row as it is stored
+    constexpr int kPer = 64 * kChunkWaves / kPieces;                                           // rows that the block loads at a time
+    constexpr int kLoads = kChunkKeys / kPer, kWords = kPiece / 4;
+    static_assert(64 / kPieces <= 16, "a wavefront's rows of a load lie among 16");
+    constexpr int kOps = D / 16, kOuts = D / 32;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];                              // [2][keys, values][64][2 D]
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int i = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x % a.p.n_kv_heads, y = blockIdx.x / a.p.n_kv_heads;
+    const Item it = item_of<kChunkRows, kChunkKeys>(a, plan, y);
+    if (it.b < 0) return;
+    const int rows = it.s.n * plan.nrep, r0 = it.set * kChunkRows, r_end = r0 + kChunkRows < rows ? r0 + kChunkRows : rows;
+    const Tiles tiles = tiles_of(it.s.pos + divide(r0, plan.rep), it.s.pos + divide(r_end - 1, plan.rep), a.p.cap, a.window, a.sinks, kChunkKeys);
+    const int parts = tiles.count > 0 ? (tiles.count - 1) / it.share + 1 : 1;
+    if (it.chunk >= parts) return;
+    const int first = parts == 1 ? 0 : it.chunk * it.share;
+    const int last = tiles.count - first < it.share ? tiles.count : first + it.share;
+    // the wavefront's rows and the lane's query (past the last: that one, not stored)
+    const int w0 = r0 + 32 * wave < r_end ? r0 + 32 * wave : r_end - 1, w_end = w0 + 32 < r_end ? w0 + 32 : r_end;
+    const bool busy = r0 + 32 * wave < r_end, live = r0 + 32 * wave + i < r_end;
+    const int row = w0 + i < w_end ? w0 + i : w_end - 1, token = divide(row, plan.rep), head = kvh * plan.nrep + (row - token * plan.nrep);
+    const int my_pos = it.s.pos + token, p_lo = it.s.pos + divide(w0, plan.rep), p_hi = it.s.pos + divide(w_end - 1, plan.rep);
+    const int before = (a.window > 0 && my_pos >= 0) ? my_pos - a.window : -1, sinks = a.window > 0 ? a.sinks : 0;
+    half8 q[kOps];
+    {
+        const uint16_t* src = a.q + (it.s.first + token) * a.ld_q + head * D + 8 * h;
+        const bool wide = reinterpret_cast<uintptr_t>(src) % 16 == 0;
+        #pragma unroll
+        for (int j = 0; j < kOps; ++j) {
+            if (wide) q[j] = *reinterpret_cast<const half8*>(src + 16 * j);
+            else
+                #pragma unroll
+                for (int e = 0; e < 8; ++e) q[j][e] = __builtin_bit_cast(_Float16, src[16 * j + e]);
+        }
+    }
+
+    // ---- a tile from its pages to registers, and from there to LDS
+    const auto* const table = reinterpret_cast<const __attribute__((address_space(4))) int*>(
+        reinterpret_cast<uintptr_t>(a.p.pages + static_cast<int64_t>(it.b) * a.p.max_pages));
+    const int my_row = wave * (64 / kPieces) + lane / kPieces, my_piece = lane % kPieces;      // of load 0; kPer rows on for the next
+    struct Raw { uint32_t k[kLoads][kWords], v[kLoads][kWords]; uint16_t ks[kLoads], vs[kLoads]; uint32_t none; } raw;
+    uint8_t* const gone = lds + chunk_lds(D);                                                  // [2][64]: keys that are not in the cache
+    struct Pages { int number[kLoads]; };
+    auto key_of = [&](int j0, int p) {             // PAGES16: of the wavefront, the first of its 16 rows; else the lane's
+        const int r = p * kPer + (PAGES16 ? (wave * (64 / kPieces) & ~15) : my_row);
+        return j0 + r < tiles.end ? j0 + r : tiles.end - 1;
+    };
+    auto look_up = [&](int v) {
+        Pages g;
+        const int j0 = tile_at(tiles, v < last ? v : last - 1) * kChunkKeys;
+        #pragma unroll
+        for (int p = 0; p < kLoads; ++p) g.number[p] = table[divide(key_of(j0, p), a.p.page)];
+        return g;
+    };
+    auto fetch = [&](int v, const Pages& g) {
+        const int j0 = tile_at(tiles, v) * kChunkKeys;
+        raw.none = 0;
+        #pragma unroll
+        for (int p = 0; p < kLoads; ++p) {
+            const int j = key_of(j0, p), number = g.number[p];
+            const bool bad = static_cast<uint32_t>(number) >= static_cast<uint32_t>(a.p.n_pages);
+            int slot = j - divide(j, a.p.page) * a.p.page.d;
+            if constexpr (PAGES16) slot &= ~15;
+            const int64_t at = row_number(a.p, bad ? 0 : number, kvh, slot);
+            const uint32_t within = PAGES16 ? my_row & 15 : 0;
+            const uint8_t *kb = a.p.k + at * kRow, *vb = a.p.v + at * kRow;
+            const uint32_t off = within * kRow + my_piece * kPiece;
+            load_words<4>(raw.k[p], kb + off);
+            load_words<4>(raw.v[p], vb + off);
+            if constexpr (kScales > 0) {
+                const uint32_t so = (within * kScales + my_piece * kScales / kPieces) * 2;
+                raw.ks[p] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.p.k_scale + at * kScales) + so);
+                raw.vs[p] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.p.v_scale + at * kScales) + so);
+            }
+            // what is not in the cache becomes zeros
+            if (bad || j0 + p * kPer + my_row >= tiles.end) raw.none |= 1u << p;
+        }
+    };
+    uint32_t exponent = 0x64006400u;
+    if constexpr (KIND == MI_KV_Q4) asm("" : "+v"(exponent));
+    auto store = [&](uint8_t* to, const uint32_t (&w)[kWords], uint16_t scale, int r) {
+        uint8_t* const line = to + r * (2 * D);
+        auto put = [&](int piece, u32x4 x) { *reinterpret_cast<u32x4*>(line + 16 * (piece ^ twist(r))) = x; };
+        if constexpr (KIND == MI_KV_F16) {
+            put(my_piece, u32x4{w[0], w[1], w[2], w[3]});
+        } else if constexpr (KIND == MI_KV_INT8) {
+            #pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                u32x4 x;
+                #pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    x[2 * z] = scaled(from_bytes<0, 1>(w[2 * e + z], w[2 * e + z]), both(scale));
+                    x[2 * z + 1] = scaled(from_bytes<2, 3>(w[2 * e + z], w[2 * e + z]), both(scale));
+                }
+                put(2 * my_piece + e, x);
+            }
+        } else {
+            #pragma unroll
+            for (int e = 0; e < kWords; ++e) {
+                uint32_t c[4];
+                #pragma unroll
+                for (int z = 0; z < 4; ++z) c[z] = scaled(from_nibbles(w[e] >> (4 * z), exponent), both(scale));
+                put(kWords * my_piece + e, u32x4{__builtin_amdgcn_perm(c[1], c[0], 0x05040100u), __builtin_amdgcn_perm(c[3], c[2], 0x05040100u),
+                                                 __builtin_amdgcn_perm(c[1], c[0], 0x07060302u), __builtin_amdgcn_perm(c[3], c[2], 0x07060302u)});
+            }
+        }
+    };
+    auto stash = [&](int buf) {
+        uint8_t* const kt = lds + buf * (chunk_lds(D) / 2);
+        if (__any(raw.none)) {
+            #pragma unroll
+            for (int p = 0; p < kLoads; ++p)
+                if (raw.none >> p & 1) {
+                    #pragma unroll
+                    for (int e = 0; e < kWords; ++e) raw.k[p][e] = raw.v[p][e] = 0;
+                    raw.ks[p] = raw.vs[p] = 0;
+                }
+        }
+        #pragma unroll
+        for (int p = 0; p < kLoads; ++p) {
+            if (my_piece == 0) gone[buf * kChunkKeys + p * kPer + my_row] = raw.none >> p & 1;
+            store(kt, raw.k[p], raw.ks[p], p * kPer + my_row);
+            store(kt + chunk_lds(D) / 4, raw.v[p], raw.vs[p], p * kPer + my_row);
+        }
+    };
+
+    floatx16 acc[kOuts];
+    #pragma unroll
+    for (int m = 0; m < kOuts; ++m)
+        #pragma unroll
+        for (int r = 0; r < 16; ++r) acc[m][r] = 0.0f;
+    float base = kStart, sum = 0.0f;               // sum: of the lane's weights, as they meet the values
+    const float scale_log2 = a.scale * 1.44269504088896341f;
+    // lane addresses within a tile: of a key operand, piece 2 j + h of row i; of a value operand, 4 rows of 16 elements for 16 lanes
+    const int vr = 4 * h + (lane & 15) / 4, vc = (lane >> 4 & 1) * 2 + (lane & 3) / 2, vo = (lane & 1) * 8;
+
+    auto multiply = [&](int v, int buf) {
+        const int j0 = tile_at(tiles, v) * kChunkKeys;
+        const uint8_t* const kt = lds + buf * (chunk_lds(D) / 2);
+        const uint8_t* const vt = kt + chunk_lds(D) / 4;
+        floatx16 s[2];
+        #pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            #pragma unroll
+            for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+            #pragma unroll
+            for (int j = 0; j < kOps; ++j)
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    *reinterpret_cast<const half8*>(kt + (32 * t + i) * (2 * D) + 16 * ((2 * j + h) ^ twist(i))), q[j], s[t], 0, 0, 0);
+        }
+        const uint64_t absent = __ballot(gone[buf * kChunkKeys + lane] != 0);
+        const bool masked = !all_seen(j0, kChunkKeys, p_lo, p_hi, a.p.cap, a.window, a.sinks) || absent != 0;
+        if (masked) {
+            asm volatile("");
+            #pragma unroll
+            for (int t = 0; t < 2; ++t)
+                #pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = j0 + 32 * t + 8 * (r / 4) + 4 * h + r % 4;
+                    const uint32_t out = static_cast<uint32_t>(absent >> (32 * t)) >> (4 * h) >> (8 * (r / 4) + r % 4) & 1;
+                    const bool see = (out == 0) & (j <= my_pos) & ((j > before) | (j < sinks));
+                    s[t][r] = see ? s[t][r] : kNone;
+                }
+        }
+        float top = max3(s[0][0], s[0][1], s[0][2]);
+        #pragma unroll
+        for (int r = 3; r < 15; r += 2) top = max3(top, s[0][r], s[0][r + 1]);
+        top = max3(top, s[0][15], s[1][0]);
+        #pragma unroll
+        for (int r = 1; r < 15; r += 2) top = max3(top, s[1][r], s[1][r + 1]);
+        top = max3(top, s[1][15], s[1][15]);
+        top = fmaf(top, scale_log2, -kHead);
+        if (__any(top > base + kSlack)) {
+            unsigned u = __float_as_uint(top);
+            const auto both_halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            top = max3(base, __uint_as_float(both_halves[0]), __uint_as_float(both_halves[1]));
+            const float alpha = __builtin_amdgcn_exp2f(base - top);
+            sum *= alpha;
+            #pragma unroll
+            for (int m = 0; m < kOuts; ++m) acc[m] *= alpha;
+            base = top;
+        }
+        uint32_t w[2][8];                          // weights, two to a word
+        #pragma unroll
+        for (int t = 0; t < 2; ++t)
+            #pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                w[t][r / 2] = pack2(__builtin_amdgcn_exp2f(fmaf(s[t][r], scale_log2, -base)), __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], scale_log2, -base)));
+                sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w[t][r / 2]), half2v{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, sum, false);
+            }
+        // operand m, keys 16 c ..: two reads of 4 keys
+        auto values = [&](int m, int c) {
+            u32x4 x;
+            #pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int r = 16 * c + 8 * z + vr;
+                const short4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
+                    vt + r * (2 * D) + 16 * ((4 * m + vc) ^ twist(r)) + vo));
+                const u32x2 two = __builtin_bit_cast(u32x2, y);
+                x[2 * z] = two[0];
+                x[2 * z + 1] = two[1];
+            }
+            return x;
+        };
+        auto weights = [&](int c) { return __builtin_bit_cast(half8, u32x4{w[c / 2][4 * (c % 2)], w[c / 2][4 * (c % 2) + 1], w[c / 2][4 * (c % 2) + 2], w[c / 2][4 * (c % 2) + 3]}); };
+        if (masked) {
+            // (a masked key's weight is 0, but 0 x inf and 0 x NaN are NaN: see paged_step_kernel)
+            uint32_t most = 0;
+            #pragma unroll
+            for (int c = 0; c < 4; ++c)
+                #pragma unroll
+                for (int m = 0; m < kOuts; ++m) {
+                    const u32x4 x = values(m, c);
+                    #pragma unroll
+                    for (int z = 0; z < 4; ++z) most |= ((x[z] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;     // exponents that are all ones
+                }
+            if (__any(most)) {
+                #pragma unroll 1
+                for (int z = 0; z < 32; ++z) {
+                    const int pos = __builtin_amdgcn_readlane(my_pos, z);
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t mask[4];
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const bool see = sees(pos, j0 + 16 * c + 8 * (e / 4) + 4 * h + e % 4, a.window, a.sinks);
+                            const uint32_t half = see ? 0xffffu << (16 * (e & 1)) : 0u;
+                            mask[e / 2] = e & 1 ? mask[e / 2] | half : half;
+                        }
+                        #pragma unroll
+                        for (int m = 0; m < kOuts; ++m) {
+                            u32x4 x = values(m, c);
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] &= mask[e];
+                            const floatx16 mine = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x), weights(c), acc[m], 0, 0, 0);
+                            if (i == z) acc[m] = mine;
+                        }
+                    }
+                }
+                return;
+            }
+        }
+        #pragma unroll
+        for (int c = 0; c < 4; ++c)
+            #pragma unroll
+            for (int m = 0; m < kOuts; ++m)
+                acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, values(m, c)), weights(c), acc[m], 0, 0, 0);
+    };
+
+    // registers -> LDS, the next tile requested, one barrier (a buffer is written again two barriers after it was last read),
+    // the tile multiplied unless the wavefront's queries see nothing of it
+    Pages pages;
+    if (first < last) {
+        pages = look_up(first);
+        fetch(first, pages);
+        pages = look_up(first + 1);
+    }
+    for (int v = first; v < last; ++v) {
+        const int buf = (v - first) & 1;
+        stash(buf);
+        if (v + 1 < last) {
+            fetch(v + 1, pages);
+            pages = look_up(v + 2);
+        }
+        __syncthreads();
+        const int j0 = tile_at(tiles, v) * kChunkKeys;
+        const int w_first = a.window > 0 && p_lo >= a.window ? p_lo - a.window + 1 : 0;        // of the window of the wavefront's first query
+        if (busy && j0 <= p_hi && (j0 + kChunkKeys > w_first || j0 < sinks)) multiply(v, buf);
+    }
+
+    if (!busy) return;
+    {
+        const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        sum = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+    }
+    if (parts > 1) {
+        // (as in paged_step_kernel, but every wavefront for its own rows)
+        constexpr int kSlot = chunk_slot_floats(D) / 2, kPairs = kOuts * 8;       // pairs of floats: of a block, of a lane
+        auto* const all = reinterpret_cast<uint64_t*>(sums);
+        const int64_t own = static_cast<int64_t>(blockIdx.x) * kSlot, zero = static_cast<int64_t>(blockIdx.x - it.chunk * a.p.n_kv_heads) * kSlot;
+        const int64_t next = static_cast<int64_t>(a.p.n_kv_heads) * kSlot;
+        const int at = wave * kPairs * 64 + lane, at_sum = kChunkWaves * kPairs * 64 + wave * 32 + i;
+        #pragma unroll
+        for (int m = 0; m < kOuts; ++m)
+            #pragma unroll
+            for (int r = 0; r < 16; r += 2)
+                __hip_atomic_store(all + own + at + (m * 8 + r / 2) * 64, __builtin_bit_cast(uint64_t, floatx2{acc[m][r], acc[m][r + 1]}),
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (h == 0)
+            __hip_atomic_store(all + own + at_sum, __builtin_bit_cast(uint64_t, floatx2{base, sum}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        uint32_t* const counter = counters + (blockIdx.x - it.chunk * a.p.n_kv_heads) * kChunkWaves + wave;
+        uint32_t arrived = 0;
+        if (lane == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (static_cast<uint32_t>(uniform(arrived)) + 1 != static_cast<uint32_t>(parts)) return;
+        asm volatile("" ::: "memory");
+        if (lane == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        auto pair_at = [&](int part, int64_t k) {
+            return __builtin_bit_cast(floatx2, __hip_atomic_load(all + zero + part * next + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+        };
+        base = kStart;
+        sum = 0.0f;
+        #pragma unroll
+        for (int m = 0; m < kOuts; ++m)
+            #pragma unroll
+            for (int r = 0; r < 16; ++r) acc[m][r] = 0.0f;
+        #pragma unroll 1
+        for (int z = 0; z < parts; ++z) {
+            const floatx2 bl = pair_at(z, at_sum);
+            floatx2 x[kPairs];
+            #pragma unroll
+            for (int k = 0; k < kPairs; ++k) x[k] = pair_at(z, at + k * 64);
+            const float now = fmaxf(base, bl[0]), was = __builtin_amdgcn_exp2f(base - now), f = __builtin_amdgcn_exp2f(bl[0] - now);
+            base = now;
+            sum = sum * was + bl[1] * f;
+            #pragma unroll
+            for (int m = 0; m < kOuts; ++m)
+                #pragma unroll
+                for (int r = 0; r < 16; ++r) acc[m][r] = acc[m][r] * was + x[m * 8 + r / 2][r & 1] * f;
+        }
+    }
+    if (!live) return;
+    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    uint16_t* const dst = a.out + (it.s.first + token) * a.ld_out + head * D + 4 * h;
+    const bool wide = reinterpret_cast<uintptr_t>(dst) % 8 == 0;
+    #pragma unroll
+    for (int m = 0; m < kOuts; ++m)
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const u32x2 x = {pack2(acc[m][4 * e] * inv, acc[m][4 * e + 1] * inv), pack2(acc[m][4 * e + 2] * inv, acc[m][4 * e + 3] * inv)};
+            uint16_t* const to = dst + 32 * m + 8 * e;
+            if (wide) {
+                *reinterpret_cast<u32x2*>(to) = x;
+            } else {
+                #pragma unroll
+                for (int z = 0; z < 4; ++z) to[z] = static_cast<uint16_t>(x[z / 2] >> (16 * (z & 1)));
+            }
+        }
+}
+
+// Blocks of a launch over sets of ROWS rows, and the plan for them: one item per set (at most one more per sequence than full
+// ones) and key/value head, and where there is a workspace for parts of sets, `want` more, as far as it reaches.
+Plan make_plan(const AttentionArgs& a, int rows_per_set, int from, int to, int want, int64_t slots, int64_t* blocks) {
     Plan plan{};
+    plan.from = from;
+    plan.to = to;
     plan.nrep = a.n_heads / a.p.n_kv_heads;
     plan.rep = make_divider(plan.nrep);
-    plan.least = 16;
-    // Sets of 16 rows: at most one more per sequence than full ones.
     const int64_t rows = static_cast<int64_t>(a.p.n_tokens) * plan.nrep, seqs = a.p.n_seqs < a.p.n_tokens ? a.p.n_seqs : a.p.n_tokens;
-    const int64_t sets = (rows - seqs) / kRows + seqs;
-    // Items beside one per set: as many blocks as the chip holds.
-    const int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (slot_floats(D) * sizeof(float))) : 0;
-    int64_t blocks = sets * a.p.n_kv_heads;
-    const int64_t want = 3 * device_info().cus, room = (slots < kSliceCounters ? slots : kSliceCounters) - blocks;
-    const int64_t target = (want < room ? want : room) / a.p.n_kv_heads;
+    const int64_t sets = (rows - seqs) / rows_per_set + seqs;
+    *blocks = sets * a.p.n_kv_heads;
+    const int64_t room = slots - *blocks, target = (want < room ? want : room) / a.p.n_kv_heads;
     plan.target = target > 0 ? static_cast<int>(target) : 0;
-    blocks += static_cast<int64_t>(plan.target) * a.p.n_kv_heads;
-    const dim3 grid(static_cast<unsigned>(blocks)), block(64 * kWaves);
+    *blocks += static_cast<int64_t>(plan.target) * a.p.n_kv_heads;
+    return plan;
+}
+
+template <int KIND, int D>
+bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to) {
+    int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (slot_floats(D) * sizeof(float))) : 0, blocks = 0;
+    if (slots > kSliceCounters) slots = kSliceCounters;
+    Plan plan = make_plan(a, kRows, 0, to, 3 * device_info().cus, slots, &blocks);
+    plan.least = 16;
     auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, grid, block, 0, s, a, plan, static_cast<float*>(workspace), workspace ? slice_counters(workspace) : nullptr);
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, a, plan, static_cast<float*>(workspace),
+                           workspace ? slice_counters(workspace) : nullptr);
     };
     if (a.p.page.d % 16 == 0) go(paged_step_kernel<KIND, D, true>);
     else go(paged_step_kernel<KIND, D, false>);
     return MI_HIP_OK(hipGetLastError());
 }
 
+template <int KIND, int D>
+bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int from) {
+    int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (chunk_slot_floats(D) * sizeof(float))) : 0, blocks = 0;
+    if (slots > kSliceCounters / kChunkWaves) slots = kSliceCounters / kChunkWaves;
+    Plan plan = make_plan(a, kChunkRows, from, 0x7fffffff, 2 * device_info().cus, slots, &blocks);
+    plan.least = 8;
+    constexpr int lds = chunk_lds(D) + 2 * kChunkKeys;
+    auto go = [&](auto kern) {
+        if (lds > 65536 && !MI_ONCE_OK(MI_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))))
+            return false;
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kChunkWaves), lds, s, a, plan, static_cast<float*>(workspace),
+                           workspace ? slice_counters(workspace) : nullptr);
+        return MI_HIP_OK(hipGetLastError());
+    };
+    return a.p.page.d % 16 == 0 ? go(paged_chunk_kernel<KIND, D, true>) : go(paged_chunk_kernel<KIND, D, false>);
+}
+
+// Sequences of up to kFew rows run on the kernel for few rows, the others on the one for many; both run where the batch may
+// have both (n_tokens and max_tokens do not say that all sequences have the same).
+constexpr int kFew = 32;
+template <int KIND, int D>
+bool launch(hipStream_t s, const AttentionArgs& a, void* workspace) {
+    const int64_t most = static_cast<int64_t>(a.max_tokens) * (a.n_heads / a.p.n_kv_heads);
+    if (most <= kFew) return launch_step<KIND, D>(s, a, workspace, 0x7fffffff);
+    if (a.p.n_seqs == 1 || static_cast<int64_t>(a.max_tokens) * a.p.n_seqs == a.p.n_tokens) return launch_chunk<KIND, D>(s, a, workspace, 0);
+    return launch_chunk<KIND, D>(s, a, workspace, kFew + 1) && launch_step<KIND, D>(s, a, workspace, kFew);
+}
+
 }  // namespace
 
 bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, void* workspace) {
     const bool wide = a.head_dim == 128;
-    if (a.kind == MI_KV_F16) return wide ? launch_step<MI_KV_F16, 128>(s, a, workspace) : launch_step<MI_KV_F16, 64>(s, a, workspace);
-    if (a.kind == MI_KV_INT8) return wide ? launch_step<MI_KV_INT8, 128>(s, a, workspace) : launch_step<MI_KV_INT8, 64>(s, a, workspace);
-    return wide ? launch_step<MI_KV_Q4, 128>(s, a, workspace) : launch_step<MI_KV_Q4, 64>(s, a, workspace);
+    if (a.kind == MI_KV_F16) return wide ? launch<MI_KV_F16, 128>(s, a, workspace) : launch<MI_KV_F16, 64>(s, a, workspace);
+    if (a.kind == MI_KV_INT8) return wide ? launch<MI_KV_INT8, 128>(s, a, workspace) : launch<MI_KV_INT8, 64>(s, a, workspace);
+    return wide ? launch<MI_KV_Q4, 128>(s, a, workspace) : launch<MI_KV_Q4, 64>(s, a, workspace);
 }
 
 }  // namespace mi
