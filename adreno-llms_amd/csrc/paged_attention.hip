@@ -38,12 +38,8 @@ __device__ __forceinline__ float max_of_groups(float a) {
     r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// (fmaxf would quieten signalling NaNs first, an instruction for each operand)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
+// The greatest of three, NaN where one is (one instruction; fmaxf would quieten signalling NaNs first, with another for each operand).
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{a, b}, half2v));
 }
@@ -71,6 +67,33 @@ __device__ __forceinline__ float sum_to_last(float x) {
     x = add_dpp<0x118, 0xf>(x);
     x = add_dpp<0x142, 0xa>(x);
     return add_dpp<0x143, 0xc>(x);
+}
+
+// A masked key has weight 0, but 0 x inf and 0 x NaN are NaN.  So in a tile that is masked for some query the values are
+// multiplied in four parts, if there are any that are not finite: the finite ones (the others as 0), and 1 for every infinity, every
+// -infinity and every NaN: the sum of a query's weights for those, where it is not 0, says that the query sees one, which is
+// then added to its output.
+__device__ __forceinline__ uint32_t odd_halves(uint32_t x) { return ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }     // top bits of odd ones
+__device__ __forceinline__ uint32_t whole_halves(uint32_t top) { return (top >> 15) * 0xffffu; }                         // top bits -> halves
+__device__ __forceinline__ uint32_t odd_part(uint32_t x, int part) {
+    const uint32_t odd = whole_halves(odd_halves(x)), nan = odd & whole_halves(((x & 0x03ff03ffu) + 0x7fff7fffu) & 0x80008000u);
+    const uint32_t sign = whole_halves(x & 0x80008000u), inf = odd & ~nan;
+    return part == 0 ? x & ~odd : (part == 1 ? inf & ~sign : part == 2 ? inf & sign : nan) & 0x3c003c00u;
+}
+__device__ __forceinline__ float with_odd(float sum, float found, int part) {
+    if (part == 0) return sum + found;
+    const float what = part == 1 ? __builtin_huge_valf() : part == 2 ? -__builtin_huge_valf() : __builtin_nanf("");
+    return found != 0.0f ? sum + what : sum;
+}
+
+// A stored element as the number it stands for.
+template <int KIND, int D>
+__device__ __forceinline__ float element(const uint8_t* pool, const uint16_t* scales, int64_t row, int e) {
+    if constexpr (KIND == MI_KV_F16) return h_f(reinterpret_cast<const uint16_t*>(pool)[row * D + e]);
+    if constexpr (KIND == MI_KV_INT8)
+        return static_cast<float>(static_cast<_Float16>(static_cast<float>(static_cast<int8_t>(pool[row * D + e])) * h_f(scales[row])));
+    const int b = pool[(row * D + e) / 2], code = (e & 1 ? b >> 4 : b & 15) - 8;
+    return static_cast<float>(static_cast<_Float16>(static_cast<float>(code) * h_f(scales[row * (D / 32) + e / 32])));
 }
 
 // ---- who does what --------------------------------------------------------------------------------------
@@ -462,7 +485,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kern
         bool masked = !all_seen(j0, kKeys, p_lo, p_hi, a.p.cap, a.window, a.sinks);
         masked |= PAGES16 ? r.absent != 0 : __any(r.absent);
         uint32_t there[4] = {};                    // halves of keys that are in the cache at all
-        if (masked) {
+        if (__builtin_expect(masked, 0)) {
             asm volatile("");                      // (a branch: most tiles are not)
             #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -475,7 +498,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kern
         }
         float top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max3(s[1][2], s[1][3], s[1][3]));
         top = fmaf(top, scale_log2, -kHead);
-        if (__any(top > base + kSlack)) {
+        if (__builtin_expect(__any(top > base + kSlack), 0)) {
             top = fmaxf(base, max_of_groups(top));
             const float alpha = __builtin_amdgcn_exp2f(base - top);
             l *= alpha;
@@ -498,36 +521,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kern
             if constexpr (more.value) load_values(next);
             return;
         }
-        // A masked key has weight 0, but 0 x inf and 0 x NaN are NaN.  What is not in the cache is taken as 0; where there is
-        // anything else that is not finite, the tile is multiplied once per query, with what that query does not see as zeros, and
-        // the query's column kept.
-        auto product = [&](int m, const uint32_t (&mask)[4]) {
+        // What is not in the cache is taken as 0; for what is and is not finite see odd_part.
+        auto product = [&](int m, floatx4 from, auto change) {
             u32x4 x;
             #pragma unroll
-            for (int p = 0; p < 4; ++p) x[p] = value_pair(t, p, m, exponent) & mask[p];
-            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, x), pb, acc[m], 0, 0, 0);
+            for (int p = 0; p < 4; ++p) x[p] = change(value_pair(t, p, m, exponent) & there[p]);
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, x), pb, from, 0, 0, 0);
         };
-        if (!__any(odd_values(t, there))) {
+        if (__builtin_expect(!__any(odd_values(t, there)), 1)) {
             #pragma unroll
-            for (int m = 0; m < kOuts; ++m) acc[m] = product(m, there);
-            if constexpr (more.value) load_values(next);
-            return;
-        }
-        #pragma unroll 1
-        for (int z = 0; z < kRows; ++z) {
-            const int pos = __builtin_amdgcn_readlane(my_pos, z);
-            uint32_t mask[4];
+            for (int m = 0; m < kOuts; ++m) acc[m] = product(m, acc[m], [](uint32_t x) { return x; });
+        } else {
             #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool see = sees(pos, j0 + 16 * (e / 4) + 4 * g + e % 4, a.window, a.sinks);
-                const uint32_t half = see ? there[e / 2] & (0xffffu << (16 * (e & 1))) : 0u;
-                mask[e / 2] = e & 1 ? mask[e / 2] | half : half;
-            }
-            #pragma unroll
-            for (int m = 0; m < kOuts; ++m) {
-                const floatx4 mine = product(m, mask);
-                if (i == z) acc[m] = mine;
-            }
+            for (int m = 0; m < kOuts; ++m)
+                #pragma unroll 1
+                for (int part = 0; part < 4; ++part) {
+                    const floatx4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const floatx4 found = product(m, none, [&](uint32_t x) { return odd_part(x, part); });
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[m][r] = with_odd(acc[m][r], found[r], part);
+                }
         }
         if constexpr (more.value) load_values(next);
     };
@@ -661,8 +674,52 @@ constexpr int chunk_slot_floats(int D) { return kChunkRows * (D + 2); }
 constexpr int chunk_lds(int D) { return 2 * 2 * kChunkKeys * 2 * D; }
 __device__ __forceinline__ constexpr int twist(int row) { return (row & 3) * 2 + (row >> 2 & 1); }
 
+// Row `q` (fp16) of a query at position pos against tiles first .. last - 1 of a sequence, one key to a lane: where an infinity or a
+// NaN in a place that some row must not see keeps the row off the matrix cores.  Leaves elements lane, lane + 64, .. of the sum of the
+// weighted values, and the sums' base.
+template <int KIND, int D>
+__device__ __forceinline__ void row_by_itself(const AttentionArgs& a, const int* table, const Tiles& tiles, int first, int last, int pos, int kvh,
+                                              const uint16_t* q, float (&o)[D / 64], float& base, float& sum) {
+    const int lane = threadIdx.x & 63;
+    base = kStart;
+    sum = 0.0f;
+    for (int d = 0; d < D / 64; ++d) o[d] = 0.0f;
+    #pragma unroll 1
+    for (int v = first; v < last; ++v) {
+        const int j = tile_at(tiles, v) * 64 + lane;
+        int lo = 0, hi = -1;                       // the key's row, in two halves; none
+        float score = kNone;
+        if (pos >= 0 && j < tiles.end && sees(pos, j, a.window, a.sinks)) {
+            const int page = divide(j, a.p.page), number = table[page];
+            if (static_cast<uint32_t>(number) < static_cast<uint32_t>(a.p.n_pages)) {
+                const int64_t at = row_number(a.p, number, kvh, j - page * a.p.page.d);
+                lo = static_cast<int>(at);
+                hi = static_cast<int>(at >> 32);
+                float dot = 0.0f;
+                #pragma unroll 1
+                for (int e = 0; e < D; ++e) dot = fmaf(h_f(q[e]), element<KIND, D>(a.p.k, a.p.k_scale, at, e), dot);
+                score = dot * a.scale * 1.44269504088896341f - kHead;
+            }
+        }
+        const float now = fmaxf(base, wave_max(score)), was = __builtin_amdgcn_exp2f(base - now);
+        const float w = hi < 0 ? 0.0f : static_cast<float>(static_cast<_Float16>(__builtin_amdgcn_exp2f(score - now)));
+        base = now;
+        sum *= was;
+        for (int d = 0; d < D / 64; ++d) o[d] *= was;
+        #pragma unroll 1
+        for (int z = 0; z < 64; ++z) {
+            const int zh = __builtin_amdgcn_readlane(hi, z);
+            if (zh < 0) continue;
+            const int64_t at = static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, z)) | static_cast<int64_t>(zh) << 32;
+            const float wz = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), z));
+            sum += wz;
+            for (int d = 0; d < D / 64; ++d) o[d] = fmaf(wz, element<KIND, D>(a.p.v, a.p.v_scale, at, lane + 64 * d), o[d]);
+        }
+    }
+}
+
 template <int KIND, int D, bool PAGES16>
-__global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ sums,
+__global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ partial,
                                                                           uint32_t* __restrict__ counters) {
     constexpr int kRow = row_bytes(KIND, D), kScales = row_scales(KIND, D);
     constexpr int kPiece = KIND == MI_KV_Q4 && D == 64 ? 8 : 16, kPieces = kRow / kPiece;      // of a row as it is stored
@@ -774,7 +831,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
     };
     auto stash = [&](int buf) {
         uint8_t* const kt = lds + buf * (chunk_lds(D) / 2);
-        if (__any(raw.none)) {
+        if (__builtin_expect(__any(raw.none), 0)) {
             #pragma unroll
             for (int p = 0; p < kLoads; ++p)
                 if (raw.none >> p & 1) {
@@ -801,6 +858,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
     // lane addresses within a tile: of a key operand, piece 2 j + h of row i; of a value operand, 4 rows of 16 elements for 16 lanes
     const int vr = 4 * h + (lane & 15) / 4, vc = (lane >> 4 & 1) * 2 + (lane & 3) / 2, vo = (lane & 1) * 8;
 
+    bool odd = false;                              // see below
     auto multiply = [&](int v, int buf) {
         const int j0 = tile_at(tiles, v) * kChunkKeys;
         const uint8_t* const kt = lds + buf * (chunk_lds(D) / 2);
@@ -817,7 +875,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
         }
         const uint64_t absent = __ballot(gone[buf * kChunkKeys + lane] != 0);
         const bool masked = !all_seen(j0, kChunkKeys, p_lo, p_hi, a.p.cap, a.window, a.sinks) || absent != 0;
-        if (masked) {
+        if (__builtin_expect(masked, 0)) {
             asm volatile("");
             #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -829,15 +887,16 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
                     s[t][r] = see ? s[t][r] : kNone;
                 }
         }
-        float top = max3(s[0][0], s[0][1], s[0][2]);
+        float tops[4];
         #pragma unroll
-        for (int r = 3; r < 15; r += 2) top = max3(top, s[0][r], s[0][r + 1]);
-        top = max3(top, s[0][15], s[1][0]);
+        for (int z = 0; z < 4; ++z) tops[z] = max3(s[z / 2][8 * (z % 2)], s[z / 2][8 * (z % 2) + 1], s[z / 2][8 * (z % 2) + 2]);
         #pragma unroll
-        for (int r = 1; r < 15; r += 2) top = max3(top, s[1][r], s[1][r + 1]);
-        top = max3(top, s[1][15], s[1][15]);
+        for (int r = 3; r < 7; r += 2)
+            #pragma unroll
+            for (int z = 0; z < 4; ++z) tops[z] = max3(tops[z], s[z / 2][8 * (z % 2) + r], s[z / 2][8 * (z % 2) + r + 1]);
+        float top = max3(max3(tops[0], s[0][7], tops[1]), max3(s[0][15], tops[2], s[1][7]), max3(tops[3], s[1][15], s[1][15]));
         top = fmaf(top, scale_log2, -kHead);
-        if (__any(top > base + kSlack)) {
+        if (__builtin_expect(__any(top > base + kSlack), 0)) {
             unsigned u = __float_as_uint(top);
             const auto both_halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);
             top = max3(base, __uint_as_float(both_halves[0]), __uint_as_float(both_halves[1]));
@@ -848,13 +907,16 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
             base = top;
         }
         uint32_t w[2][8];                          // weights, two to a word
+        float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
         #pragma unroll
         for (int t = 0; t < 2; ++t)
             #pragma unroll
             for (int r = 0; r < 16; r += 2) {
                 w[t][r / 2] = pack2(__builtin_amdgcn_exp2f(fmaf(s[t][r], scale_log2, -base)), __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], scale_log2, -base)));
-                sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w[t][r / 2]), half2v{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, sum, false);
+                float& part = sums[2 * t + r / 2 % 2];
+                part = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w[t][r / 2]), half2v{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, part, false);
             }
+        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
         // operand m, keys 16 c ..: two reads of 4 keys
         auto values = [&](int m, int c) {
             u32x4 x;
@@ -870,8 +932,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
             return x;
         };
         auto weights = [&](int c) { return __builtin_bit_cast(half8, u32x4{w[c / 2][4 * (c % 2)], w[c / 2][4 * (c % 2) + 1], w[c / 2][4 * (c % 2) + 2], w[c / 2][4 * (c % 2) + 3]}); };
-        if (masked) {
-            // (a masked key's weight is 0, but 0 x inf and 0 x NaN are NaN: see paged_step_kernel)
+        if (__builtin_expect(masked, 0)) {
+            // A masked key has weight 0, but 0 x inf and 0 x NaN are NaN: where there is an infinity or a NaN in a tile that is masked
+            // for some query, the wavefront does its rows again in the end (redo), whatever comes out here.
             uint32_t most = 0;
             #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -879,33 +942,9 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
                 for (int m = 0; m < kOuts; ++m) {
                     const u32x4 x = values(m, c);
                     #pragma unroll
-                    for (int z = 0; z < 4; ++z) most |= ((x[z] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;     // exponents that are all ones
+                    for (int z = 0; z < 4; ++z) most |= odd_halves(x[z]);
                 }
-            if (__any(most)) {
-                #pragma unroll 1
-                for (int z = 0; z < 32; ++z) {
-                    const int pos = __builtin_amdgcn_readlane(my_pos, z);
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t mask[4];
-                        #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const bool see = sees(pos, j0 + 16 * c + 8 * (e / 4) + 4 * h + e % 4, a.window, a.sinks);
-                            const uint32_t half = see ? 0xffffu << (16 * (e & 1)) : 0u;
-                            mask[e / 2] = e & 1 ? mask[e / 2] | half : half;
-                        }
-                        #pragma unroll
-                        for (int m = 0; m < kOuts; ++m) {
-                            u32x4 x = values(m, c);
-                            #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] &= mask[e];
-                            const floatx16 mine = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x), weights(c), acc[m], 0, 0, 0);
-                            if (i == z) acc[m] = mine;
-                        }
-                    }
-                }
-                return;
-            }
+            odd |= __any(most) != 0;
         }
         #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -936,25 +975,47 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
     }
 
     if (!busy) return;
-    {
+    constexpr int kSlot = chunk_slot_floats(D) / 2, kPairs = kOuts * 8;           // pairs of floats: of a block, of a lane
+    auto* const all = reinterpret_cast<uint64_t*>(partial);
+    const int64_t own = static_cast<int64_t>(blockIdx.x) * kSlot;
+    const int at = wave * kPairs * 64 + lane, at_sum = kChunkWaves * kPairs * 64 + wave * 32 + i;
+    if (__builtin_expect(odd, 0)) {
+        #pragma unroll 1
+        for (int z = 0; z < 32 && w0 + z < w_end; ++z) {
+            const int r = w0 + z, t = divide(r, plan.rep), hd = kvh * plan.nrep + (r - t * plan.nrep);
+            float o[D / 64], b, l;
+            row_by_itself<KIND, D>(a, a.p.pages + static_cast<int64_t>(it.b) * a.p.max_pages, tiles, first, last, it.s.pos + t, kvh, a.q + (it.s.first + t) * a.ld_q + hd * D, o, b, l);
+            #pragma unroll
+            for (int e = 0; e < D / 64; ++e) {
+                const int d = lane + 64 * e, reg = 4 * (d % 32 / 8) + d % 4, place = (d / 4 % 2) * 32 + z;   // as the others lie in the registers
+                if (parts == 1)
+                    a.out[(it.s.first + t) * a.ld_out + hd * D + d] = f_h(l == 0.0f ? 0.0f : o[e] / l);
+                else
+                    __hip_atomic_store(reinterpret_cast<float*>(all + own + wave * kPairs * 64 + (d / 32 * 8 + reg / 2) * 64 + place) + reg % 2, o[e],
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            if (parts > 1 && lane == 0)
+                __hip_atomic_store(all + own + kChunkWaves * kPairs * 64 + wave * 32 + z, __builtin_bit_cast(uint64_t, floatx2{b, l}), __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (parts == 1) return;
+    } else {
         const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
         sum = __uint_as_float(halves[0]) + __uint_as_float(halves[1]);
+        if (parts > 1) {
+            // (as in paged_step_kernel, but every wavefront for its own rows)
+            #pragma unroll
+            for (int m = 0; m < kOuts; ++m)
+                #pragma unroll
+                for (int r = 0; r < 16; r += 2)
+                    __hip_atomic_store(all + own + at + (m * 8 + r / 2) * 64, __builtin_bit_cast(uint64_t, floatx2{acc[m][r], acc[m][r + 1]}),
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (h == 0)
+                __hip_atomic_store(all + own + at_sum, __builtin_bit_cast(uint64_t, floatx2{base, sum}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
     if (parts > 1) {
-        // (as in paged_step_kernel, but every wavefront for its own rows)
-        constexpr int kSlot = chunk_slot_floats(D) / 2, kPairs = kOuts * 8;       // pairs of floats: of a block, of a lane
-        auto* const all = reinterpret_cast<uint64_t*>(sums);
-        const int64_t own = static_cast<int64_t>(blockIdx.x) * kSlot, zero = static_cast<int64_t>(blockIdx.x - it.chunk * a.p.n_kv_heads) * kSlot;
-        const int64_t next = static_cast<int64_t>(a.p.n_kv_heads) * kSlot;
-        const int at = wave * kPairs * 64 + lane, at_sum = kChunkWaves * kPairs * 64 + wave * 32 + i;
-        #pragma unroll
-        for (int m = 0; m < kOuts; ++m)
-            #pragma unroll
-            for (int r = 0; r < 16; r += 2)
-                __hip_atomic_store(all + own + at + (m * 8 + r / 2) * 64, __builtin_bit_cast(uint64_t, floatx2{acc[m][r], acc[m][r + 1]}),
-                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (h == 0)
-            __hip_atomic_store(all + own + at_sum, __builtin_bit_cast(uint64_t, floatx2{base, sum}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int64_t zero_at = static_cast<int64_t>(blockIdx.x - it.chunk * a.p.n_kv_heads) * kSlot, next = static_cast<int64_t>(a.p.n_kv_heads) * kSlot;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         uint32_t* const counter = counters + (blockIdx.x - it.chunk * a.p.n_kv_heads) * kChunkWaves + wave;
         uint32_t arrived = 0;
@@ -963,7 +1024,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
         asm volatile("" ::: "memory");
         if (lane == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         auto pair_at = [&](int part, int64_t k) {
-            return __builtin_bit_cast(floatx2, __hip_atomic_load(all + zero + part * next + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            return __builtin_bit_cast(floatx2, __hip_atomic_load(all + zero_at + part * next + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
         };
         base = kStart;
         sum = 0.0f;

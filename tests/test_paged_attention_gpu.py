@@ -66,22 +66,22 @@ def test_what_a_masked_position_holds_does_not_matter(queue, kind, form):
     """NaN and infinities in a chunk's later rows, which earlier rows of the same tile must not take up, and in
     positions behind the window."""
     c = Cache(kind, 14, 2, 64, 16, seed=7, **form)
-    m = c.lengths[0]
-    clean = Cache(kind, 14, 2, 64, 16, seed=7, **form).upload().attend(queue)
+    m, n = c.lengths[0], c.new[0]
     for name, bad in ((c.k, np.nan), (c.v, np.inf), (c.v, np.nan)):
         name[0][m - 5, :, 11] = bad
     c.fill()
     c.upload()
-    rows = c.new[0] - 5 if c.new[0] > 5 else 0
     got = c.attend(queue)
-    assert np.array_equal(got[:rows].view(np.uint16), clean[:rows].view(np.uint16))
-    assert np.isnan(got[c.new[0] - 1]).any()
-    if len(c.new) > 1:
-        assert np.array_equal(got[c.new[0]:].view(np.uint16), clean[c.new[0]:].view(np.uint16))
-    # with a window of 3 the last two rows do not see the position any more (NaN where a row does)
+    # the rows that do not see it: as ever.  (Not bit for bit what they are without it: a row that shares a tile with such a place may
+    # be summed in another order; the tolerance holds for any.)
+    unseen = np.r_[0:max(n - 5, 0), n:sum(c.new)]
+    c.check(got, rows=unseen)
+    assert np.isnan(got[n - 1]).any()
+    # with a window of 3 the last two rows do not see the position any more
     got = c.attend(queue, window=3)
-    want = Cache(kind, 14, 2, 64, 16, seed=7, **form).upload().attend(queue, window=3)
-    assert np.array_equal(got[c.new[0] - 1].view(np.uint16), want[c.new[0] - 1].view(np.uint16))
+    c.check(got, window=3, rows=np.r_[0:max(n - 5, 0), max(n - 2, 0):n])
+    if n > 2:
+        assert np.isnan(got[n - 3]).any() and np.isnan(got[n - 5]).any()
 
 
 def test_infinite_values_that_are_seen(queue):
