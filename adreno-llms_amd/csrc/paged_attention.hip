@@ -671,7 +671,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kern
 
 constexpr int kChunkKeys = 64, kChunkWaves = 4, kChunkRows = 32 * kChunkWaves;
 constexpr int chunk_slot_floats(int D) { return kChunkRows * (D + 2); }
-constexpr int chunk_lds(int D) { return 2 * 2 * kChunkKeys * 2 * D; }
+constexpr int chunk_lds(int D) { return 2 * 2 * kChunkKeys * 2 * D; }          // of a slice's tiles
+constexpr int chunk_lds_all(int D, int KS) { return KS * (chunk_lds(D) + 2 * kChunkKeys); }
+constexpr int meet_bytes(int D) { return kChunkWaves * 64 * (D / 2 + 3) * 4; }    // of a slice's sums
 __device__ __forceinline__ constexpr int twist(int row) { return (row & 3) * 2 + (row >> 2 & 1); }
 
 // Row `q` (fp16) of a query at position pos against tiles first .. last - 1 of a sequence, one key to a lane: where an infinity or a
@@ -718,8 +720,8 @@ __device__ __forceinline__ void row_by_itself(const AttentionArgs& a, const int*
     }
 }
 
-template <int KIND, int D, bool PAGES16>
-__global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ partial,
+template <int KIND, int D, bool PAGES16, int KS>
+__global__ __launch_bounds__(64 * kChunkWaves * KS, 2) void paged_chunk_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ partial,
                                                                           uint32_t* __restrict__ counters) {
     constexpr int kRow = row_bytes(KIND, D), kScales = row_scales(KIND, D);
     constexpr int kPiece = KIND == MI_KV_Q4 && D == 64 ? 8 : 16, kPieces = kRow / kPiece;      // of a row as it is stored
@@ -728,7 +730,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
     static_assert(64 / kPieces <= 16, "a wavefront's rows of a load lie among 16");
     constexpr int kOps = D / 16, kOuts = D / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];                              // [2][keys, values][64][2 D]
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6) % kChunkWaves, slice = uniform(tid >> 6) / kChunkWaves;
     const int i = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x % a.p.n_kv_heads, y = blockIdx.x / a.p.n_kv_heads;
     const Item it = item_of<kChunkRows, kChunkKeys>(a, plan, y);
@@ -763,7 +765,8 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
         reinterpret_cast<uintptr_t>(a.p.pages + static_cast<int64_t>(it.b) * a.p.max_pages));
     const int my_row = wave * (64 / kPieces) + lane / kPieces, my_piece = lane % kPieces;      // of load 0; kPer rows on for the next
     struct Raw { uint32_t k[kLoads][kWords], v[kLoads][kWords]; uint16_t ks[kLoads], vs[kLoads]; uint32_t none; } raw;
-    uint8_t* const gone = lds + chunk_lds(D);                                                  // [2][64]: keys that are not in the cache
+    uint8_t* const own_lds = lds + slice * chunk_lds(D);
+    uint8_t* const gone = lds + KS * chunk_lds(D) + slice * 2 * kChunkKeys;                                                  // [2][64]: keys that are not in the cache
     struct Pages { int number[kLoads]; };
     auto key_of = [&](int j0, int p) {             // PAGES16: of the wavefront, the first of its 16 rows; else the lane's
         const int r = p * kPer + (PAGES16 ? (wave * (64 / kPieces) & ~15) : my_row);
@@ -830,7 +833,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
         }
     };
     auto stash = [&](int buf) {
-        uint8_t* const kt = lds + buf * (chunk_lds(D) / 2);
+        uint8_t* const kt = own_lds + buf * (chunk_lds(D) / 2);
         if (__builtin_expect(__any(raw.none), 0)) {
             #pragma unroll
             for (int p = 0; p < kLoads; ++p)
@@ -861,7 +864,7 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
     bool odd = false;                              // see below
     auto multiply = [&](int v, int buf) {
         const int j0 = tile_at(tiles, v) * kChunkKeys;
-        const uint8_t* const kt = lds + buf * (chunk_lds(D) / 2);
+        const uint8_t* const kt = own_lds + buf * (chunk_lds(D) / 2);
         const uint8_t* const vt = kt + chunk_lds(D) / 4;
         floatx16 s[2];
         #pragma unroll
@@ -955,25 +958,52 @@ __global__ __launch_bounds__(64 * kChunkWaves, 2) void paged_chunk_kernel(const 
 
     // registers -> LDS, the next tile requested, one barrier (a buffer is written again two barriers after it was last read),
     // the tile multiplied unless the wavefront's queries see nothing of it
+    // (of KS slices: tiles first + slice, + KS, ..; past the last that one again, not multiplied)
     Pages pages;
+    const int mine = first + slice;
+    auto clamp = [&](int v) { return v < last ? v : last - 1; };
     if (first < last) {
-        pages = look_up(first);
-        fetch(first, pages);
-        pages = look_up(first + 1);
+        pages = look_up(mine);
+        fetch(clamp(mine), pages);
+        pages = look_up(mine + KS);
     }
-    for (int v = first; v < last; ++v) {
-        const int buf = (v - first) & 1;
+    for (int v = mine, buf = 0; v - slice < last; v += KS, buf ^= 1) {
         stash(buf);
-        if (v + 1 < last) {
-            fetch(v + 1, pages);
-            pages = look_up(v + 2);
+        if (v - slice + KS < last) {
+            fetch(clamp(v + KS), pages);
+            pages = look_up(v + 2 * KS);
         }
         __syncthreads();
-        const int j0 = tile_at(tiles, v) * kChunkKeys;
-        const int w_first = a.window > 0 && p_lo >= a.window ? p_lo - a.window + 1 : 0;        // of the window of the wavefront's first query
-        if (busy && j0 <= p_hi && (j0 + kChunkKeys > w_first || j0 < sinks)) multiply(v, buf);
+        if (v < last) {
+            const int j0 = tile_at(tiles, v) * kChunkKeys;
+            const int w_first = a.window > 0 && p_lo >= a.window ? p_lo - a.window + 1 : 0;    // of the window of the wavefront's first query
+            if (busy && j0 <= p_hi && (j0 + kChunkKeys > w_first || j0 < sinks)) multiply(v, buf);
+        }
     }
-
+    if constexpr (KS == 2) {
+        // The second slice's sums come to the first by LDS.
+        __syncthreads();
+        float* const box = reinterpret_cast<float*>(lds) + wave * 64 * (D / 2 + 3) + lane;
+        if (slice == 1) {
+            box[0] = base;
+            box[64] = sum;
+            box[128] = odd ? 1.0f : 0.0f;
+            #pragma unroll
+            for (int m = 0; m < kOuts; ++m)
+                #pragma unroll
+                for (int r = 0; r < 16; ++r) box[(3 + 16 * m + r) * 64] = acc[m][r];
+        }
+        __syncthreads();
+        if (slice == 1) return;
+        const float now = fmaxf(base, box[0]), was = __builtin_amdgcn_exp2f(base - now), f = __builtin_amdgcn_exp2f(box[0] - now);
+        base = now;
+        sum = sum * was + box[64] * f;
+        odd |= __any(box[128] != 0.0f) != 0;
+        #pragma unroll
+        for (int m = 0; m < kOuts; ++m)
+            #pragma unroll
+            for (int r = 0; r < 16; ++r) acc[m][r] = acc[m][r] * was + box[(3 + 16 * m + r) * 64] * f;
+    }
     if (!busy) return;
     constexpr int kSlot = chunk_slot_floats(D) / 2, kPairs = kOuts * 8;           // pairs of floats: of a block, of a lane
     auto* const all = reinterpret_cast<uint64_t*>(partial);
@@ -1098,21 +1128,36 @@ bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to)
     return MI_HIP_OK(hipGetLastError());
 }
 
+template <int KIND, int D, int KS>
+bool launch_slices(hipStream_t s, const AttentionArgs& a, const Plan& plan, int64_t blocks, void* workspace) {
+    constexpr int lds = chunk_lds_all(D, KS);
+    static_assert(lds <= 160 * 1024 && (KS == 1 || meet_bytes(D) <= KS * chunk_lds(D)), "tiles and sums fit");
+    auto go = [&](auto kern) {
+        if (lds > 65536 && !MI_ONCE_OK(MI_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))))
+            return false;
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kChunkWaves * KS), lds, s, a, plan, static_cast<float*>(workspace),
+                           workspace ? slice_counters(workspace) : nullptr);
+        return MI_HIP_OK(hipGetLastError());
+    };
+    return a.p.page.d % 16 == 0 ? go(paged_chunk_kernel<KIND, D, true, KS>) : go(paged_chunk_kernel<KIND, D, false, KS>);
+}
+
 template <int KIND, int D>
 bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int from) {
     int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (chunk_slot_floats(D) * sizeof(float))) : 0, blocks = 0;
     if (slots > kSliceCounters / kChunkWaves) slots = kSliceCounters / kChunkWaves;
-    Plan plan = make_plan(a, kChunkRows, from, 0x7fffffff, 2 * device_info().cus, slots, &blocks);
-    plan.least = 8;
-    constexpr int lds = chunk_lds(D) + 2 * kChunkKeys;
-    auto go = [&](auto kern) {
-        if (lds > 65536 && !MI_ONCE_OK(MI_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))))
-            return false;
-        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kChunkWaves), lds, s, a, plan, static_cast<float*>(workspace),
-                           workspace ? slice_counters(workspace) : nullptr);
-        return MI_HIP_OK(hipGetLastError());
-    };
-    return a.p.page.d % 16 == 0 ? go(paged_chunk_kernel<KIND, D, true>) : go(paged_chunk_kernel<KIND, D, false>);
+    int64_t sets = 0;
+    (void)make_plan(a, kChunkRows, from, 0x7fffffff, 0, 0, &sets);
+    // A block of eight wavefronts, two slices of a set's keys, is alone on its CU; of four wavefronts there are two.  So few sets
+    // are taken in two slices (us with / without: 300 rows of 14 heads at 900 int8 15.0 / 15.3, width 128 in 17 conversations, 208 sets,
+    // 100 / 125) and many are not (2048 rows of 14 heads, 224 sets, 33.7 / 29.7: a second round); wide heads, where a wavefront's tile takes
+    // twice as long, up to more of them.  Parts of sets meet in memory as well, as many as blocks are resident.
+    const int64_t cus = device_info().cus;
+    const bool two = sets <= (D == 128 ? cus * 3 / 2 : cus / 2);
+    const int64_t want = two ? (sets < cus ? cus - sets : 0) : 2 * cus;
+    Plan plan = make_plan(a, kChunkRows, from, 0x7fffffff, static_cast<int>(want), slots, &blocks);
+    plan.least = 4;
+    return two ? launch_slices<KIND, D, 2>(s, a, plan, blocks, workspace) : launch_slices<KIND, D, 1>(s, a, plan, blocks, workspace);
 }
 
 // Sequences of up to kFew rows run on the kernel for few rows, the others on the one for many; both run where the batch may
