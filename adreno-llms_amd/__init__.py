@@ -408,7 +408,7 @@ class KVCache(C.Structure):
 
     def __init__(self, kind, n_pages, page_size, n_kv_heads, head_dim, k, v, k_scale=None, v_scale=None):
         super().__init__(_h(k), _h(v), _h(k_scale), _h(v_scale), kind, n_pages, page_size, n_kv_heads, head_dim)
-        self._keep = (k, v, k_scale, v_scale)
+        self._keep, self._at = (k, v, k_scale, v_scale), C.addressof(self)
 
 
 class KVBatch(C.Structure):
@@ -419,7 +419,7 @@ class KVBatch(C.Structure):
 
     def __init__(self, n_seqs, n_tokens, max_tokens, max_pages, q_start, kv_len, pages):
         super().__init__(_h(q_start), _h(kv_len), _h(pages), n_seqs, n_tokens, max_tokens, max_pages)
-        self._keep = (q_start, kv_len, pages)
+        self._keep, self._at = (q_start, kv_len, pages), C.addressof(self)
 
 
 class AttentionCall(C.Structure):
@@ -432,25 +432,25 @@ class AttentionCall(C.Structure):
         width = n_heads * cache.head_dim
         super().__init__(C.pointer(cache), C.pointer(batch), _h(q), _h(out), ld_q or width, ld_out or width, n_heads,
                          cache.head_dim ** -0.5 if scale is None else scale, window, sinks)
-        self._keep = (cache, batch, q, out)
+        self._keep, self._at = (cache, batch, q, out), C.addressof(self)
 
 
 def kv_write(queue, cache, batch, k, v, ld_k=0, ld_v=0):
     """New tokens' keys and values into their pages (mi_kv_write); ld_k, ld_v: 0 for n_kv_heads * head_dim."""
     width = cache.n_kv_heads * cache.head_dim
-    return bool(lib().mi_kv_write(_q(queue), C.addressof(cache), C.addressof(batch), _h(k), ld_k or width, _h(v), ld_v or width))
+    return bool(lib().mi_kv_write(_q(queue), cache._at, batch._at, _h(k), ld_k or width, _h(v), ld_v or width))
 
 
 def kv_read(queue, cache, batch, k_out, v_out, ld_k=0, ld_v=0):
     """The same rows back out of their pages, as fp16 (mi_kv_read)."""
     width = cache.n_kv_heads * cache.head_dim
-    return bool(lib().mi_kv_read(_q(queue), C.addressof(cache), C.addressof(batch), _h(k_out), ld_k or width, _h(v_out),
+    return bool(lib().mi_kv_read(_q(queue), cache._at, batch._at, _h(k_out), ld_k or width, _h(v_out),
                                  ld_v or width))
 
 
 def attention(queue, call):
     """Attention of the new tokens over the cache (mi_attention)."""
-    return bool(lib().mi_attention(_q(queue), C.addressof(call)))
+    return bool(lib().mi_attention(_q(queue), call._at))
 
 
 # ------------------------------------------------------------------- offline tools

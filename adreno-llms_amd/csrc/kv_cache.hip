@@ -21,33 +21,34 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 256;
 constexpr int kPiece = 8;                          // values per thread: 16 bytes of an fp16 row
 
-// Where a thread's 8 values are: row of the batch, head, first element, and the row's number in the pools (-1: it has no place).
+// Where row `row` of the batch lies in the cache: the number of its row of head 0 in the pools (the next head's is a page further), -1
+// where it has no place.  `mine`: it belongs to a sequence.  The same for a wavefront; its lanes look for the sequence together, as
+// a search by halves would wait for a load at every step.
 struct Place {
-    int row, head, at;
     int64_t cache;
-    bool mine;                                     // the row belongs to a sequence
+    bool mine;
 };
-template <int D>
-__device__ __forceinline__ Place place_of(const PagedArgs& a) {
-    constexpr int kPieces = D / kPiece;
-    const int64_t id = static_cast<int64_t>(blockIdx.x) * (kThreads / kPieces) + threadIdx.x / kPieces;
-    Place p{};
-    p.cache = -1;
-    p.row = static_cast<int>(id / a.n_kv_heads);
-    p.head = static_cast<int>(id % a.n_kv_heads);
-    p.at = static_cast<int>(threadIdx.x % kPieces) * kPiece;
-    if (p.row >= a.n_tokens) return p;
-    const int b = sequence_of(a.q_start, a.n_seqs, p.row);
+__device__ __forceinline__ Place place_of(const PagedArgs& a, int row) {
+    Place p{-1, false};
+    const int lane = threadIdx.x & 63;
+    int b = -1;
+    for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
+        const int s = b0 + lane < a.n_seqs ? b0 + lane : a.n_seqs - 1;
+        const int here = __popcll(__ballot(b0 + lane < a.n_seqs && a.q_start[s] <= row));
+        b += here;
+        if (here < 64) break;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
     if (b < 0) return p;
     const Span s = span_of(a.q_start[b], a.q_start[b + 1], a.kv_len[b], a.n_tokens);
-    if (p.row - s.first >= s.n) return p;
+    if (row < s.first || row - s.first >= s.n) return p;
     p.mine = true;
-    const int pos = s.pos + (p.row - s.first);
+    const int pos = s.pos + (row - s.first);
     if (pos < 0 || pos >= a.cap) return p;
     const int page = divide(pos, a.page);
-    const int number = a.pages[static_cast<int64_t>(b) * a.max_pages + page];
-    if (number < 0 || number >= a.n_pages) return p;
-    p.cache = row_number(a, number, p.head, pos - page * a.page.d);
+    const int number = __builtin_amdgcn_readfirstlane(a.pages[static_cast<int64_t>(b) * a.max_pages + page]);
+    if (static_cast<uint32_t>(number) >= static_cast<uint32_t>(a.n_pages)) return p;
+    p.cache = row_number(a, number, 0, pos - page * a.page.d);
     return p;
 }
 
@@ -61,104 +62,126 @@ __device__ __forceinline__ float max_of(float m) {
     return m;
 }
 
-// blockIdx.y: keys, values.  Bound by bytes where there are many rows (16 in and 16, 8 or 4 out per thread), by the chain
-// of loads to a row's place (q_start, kv_len, pages) where there are few.
+// A wavefront has one row of keys or values (blockIdx.y), 512 of its elements at a time, 8 to a lane.  Bound by bytes where there
+// are many rows, by the chain of loads to a row's place (q_start, kv_len, pages) where there are few.  A thread for every 8
+// elements that looked its place up by itself took 42 us to read 6 Q4 conversations of up to 8000 (102 MB).
 template <int KIND, int D>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const PagedArgs a, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                             const int64_t ld_k, const int64_t ld_v) {
-    const Place p = place_of<D>(a);
-    if (p.cache < 0) return;                       // (all lanes of a row alike)
-    const uint16_t* src = blockIdx.y ? v + p.row * ld_v : k + p.row * ld_k;
-    src += p.head * D + p.at;
-    half8 x;
-    if (reinterpret_cast<uintptr_t>(src) % 16 == 0) x = *reinterpret_cast<const half8*>(src);
-    else
+    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (row >= a.n_tokens) return;
+    const uint16_t* const src = blockIdx.y ? v + row * ld_v : k + row * ld_k;
+    const bool wide = reinterpret_cast<uintptr_t>(src) % 16 == 0;
+    const int width = a.n_kv_heads * D;
+    // (the first elements are on their way while the row's place is looked up)
+    auto load = [&](int e0) {
+        half8 x = {};
+        const int e = e0 + kPiece * lane;
+        if (e >= width) return x;
+        if (wide) return *reinterpret_cast<const half8*>(src + e);
         #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __builtin_bit_cast(_Float16, src[e]);
+        for (int z = 0; z < 8; ++z) x[z] = __builtin_bit_cast(_Float16, src[e + z]);
+        return x;
+    };
+    half8 x = load(0);
+    const Place p = place_of(a, row);
+    if (p.cache < 0) return;
     uint8_t* const pool = const_cast<uint8_t*>(blockIdx.y ? a.v : a.k);
-    if constexpr (KIND == MI_KV_F16) {
-        *reinterpret_cast<half8*>(pool + (p.cache * D + p.at) * 2) = x;
-    } else {
-        constexpr bool kInt8 = KIND == MI_KV_INT8;
-        constexpr float kTop = kInt8 ? 127.0f : 7.0f, kMost = kInt8 ? 515.5f : 9352.0f;     // (code * scale stays below 65520)
-        // 0 for all finite values, else NaN: a NaN would be lost among maxima
-        float big = 0.0f, bad = 0.0f;
-        #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float f = static_cast<float>(x[e]);
-            big = fmaxf(big, fabsf(f));
-            bad += f * 0.0f;
+    uint16_t* const scales = const_cast<uint16_t*>(blockIdx.y ? a.v_scale : a.k_scale);
+    for (int e0 = 0; e0 < width; e0 += 64 * kPiece) {
+        const half8 next = load(e0 + 64 * kPiece);
+        const int e = e0 + kPiece * lane, at = e % D;
+        const int64_t cache = p.cache + static_cast<int64_t>(e / D) * a.page.d;
+        if (e < width) {
+            if constexpr (KIND == MI_KV_F16) {
+                *reinterpret_cast<half8*>(pool + (cache * D + at) * 2) = x;
+            } else {
+                constexpr bool kInt8 = KIND == MI_KV_INT8;
+                constexpr float kTop = kInt8 ? 127.0f : 7.0f, kMost = kInt8 ? 515.5f : 9352.0f;     // (code * scale stays below 65520)
+                // 0 for all finite values, else NaN: a NaN would be lost among maxima
+                float big = 0.0f, bad = 0.0f;
+                #pragma unroll
+                for (int z = 0; z < 8; ++z) {
+                    const float f = static_cast<float>(x[z]);
+                    big = fmaxf(big, fabsf(f));
+                    bad += f * 0.0f;
+                }
+                if (bad != 0.0f) big = __builtin_huge_valf();
+                big = max_of<kInt8 ? D / kPiece : 32 / kPiece>(big);
+                const bool finite = big <= 65504.0f;
+                const _Float16 h = static_cast<_Float16>(finite ? fminf(__fdiv_rn(big, kTop), kMost) : __builtin_nanf(""));
+                const float scale = static_cast<float>(h);
+                int code[8];
+                #pragma unroll
+                for (int z = 0; z < 8; ++z) {
+                    const float c = finite && scale > 0.0f ? rintf(__fdiv_rn(static_cast<float>(x[z]), scale)) : 0.0f;
+                    code[z] = static_cast<int>(fminf(fmaxf(c, kInt8 ? -127.0f : -8.0f), kTop));
+                }
+                if constexpr (kInt8) {
+                    u32x2 w = {0, 0};
+                    #pragma unroll
+                    for (int z = 0; z < 8; ++z) w[z / 4] |= static_cast<uint32_t>(code[z] & 255) << (8 * (z % 4));
+                    *reinterpret_cast<u32x2*>(pool + cache * D + at) = w;
+                    if (at == 0) scales[cache] = __builtin_bit_cast(uint16_t, h);
+                } else {
+                    uint32_t w = 0;
+                    #pragma unroll
+                    for (int z = 0; z < 8; ++z) w |= static_cast<uint32_t>(code[z] + 8) << (4 * z);
+                    *reinterpret_cast<uint32_t*>(pool + (cache * D + at) / 2) = w;
+                    if (at % 32 == 0) scales[cache * (D / 32) + at / 32] = __builtin_bit_cast(uint16_t, h);
+                }
+            }
         }
-        if (bad != 0.0f) big = __builtin_huge_valf();
-        big = max_of<kInt8 ? D / kPiece : 32 / kPiece>(big);
-        const bool finite = big <= 65504.0f;
-        const _Float16 h = static_cast<_Float16>(finite ? fminf(__fdiv_rn(big, kTop), kMost) : __builtin_nanf(""));
-        const float scale = static_cast<float>(h);
-        int code[8];
-        #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float c = finite && scale > 0.0f ? rintf(__fdiv_rn(static_cast<float>(x[e]), scale)) : 0.0f;
-            code[e] = static_cast<int>(fminf(fmaxf(c, kInt8 ? -127.0f : -8.0f), kTop));
-        }
-        uint16_t* const scales = const_cast<uint16_t*>(blockIdx.y ? a.v_scale : a.k_scale);
-        if constexpr (kInt8) {
-            u32x2 w = {0, 0};
-            #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e / 4] |= static_cast<uint32_t>(code[e] & 255) << (8 * (e % 4));
-            *reinterpret_cast<u32x2*>(pool + p.cache * D + p.at) = w;
-            if (p.at == 0) scales[p.cache] = __builtin_bit_cast(uint16_t, h);
-        } else {
-            uint32_t w = 0;
-            #pragma unroll
-            for (int e = 0; e < 8; ++e) w |= static_cast<uint32_t>(code[e] + 8) << (4 * e);
-            *reinterpret_cast<uint32_t*>(pool + (p.cache * D + p.at) / 2) = w;
-            if (p.at % 32 == 0) scales[p.cache * (D / 32) + p.at / 32] = __builtin_bit_cast(uint16_t, h);
-        }
+        x = next;
     }
 }
 
 template <int KIND, int D>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(const PagedArgs a, uint16_t* __restrict__ k, uint16_t* __restrict__ v,
                                                            const int64_t ld_k, const int64_t ld_v) {
-    const Place p = place_of<D>(a);
+    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (row >= a.n_tokens) return;
+    const Place p = place_of(a, row);
     if (!p.mine) return;
-    half8 x;
-    #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = static_cast<_Float16>(0.0f);
-    if (p.cache >= 0) {
-        const uint8_t* const pool = blockIdx.y ? a.v : a.k;
-        if constexpr (KIND == MI_KV_F16) {
-            x = *reinterpret_cast<const half8*>(pool + (p.cache * D + p.at) * 2);
-        } else {
-            const uint16_t* const scales = blockIdx.y ? a.v_scale : a.k_scale;
-            if constexpr (KIND == MI_KV_INT8) {
-                const float scale = h_f(scales[p.cache]);
-                const u32x2 w = *reinterpret_cast<const u32x2*>(pool + p.cache * D + p.at);
+    uint16_t* const dst = blockIdx.y ? v + row * ld_v : k + row * ld_k;
+    const bool wide = reinterpret_cast<uintptr_t>(dst) % 16 == 0;
+    const uint8_t* const pool = blockIdx.y ? a.v : a.k;
+    const uint16_t* const scales = blockIdx.y ? a.v_scale : a.k_scale;
+    const int width = a.n_kv_heads * D;
+    #pragma unroll 2
+    for (int e = kPiece * lane; e < width; e += 64 * kPiece) {
+        const int at = e % D;
+        const int64_t cache = p.cache + static_cast<int64_t>(e / D) * a.page.d;
+        half8 x = {};
+        if (p.cache >= 0) {
+            if constexpr (KIND == MI_KV_F16) {
+                x = *reinterpret_cast<const half8*>(pool + (cache * D + at) * 2);
+            } else if constexpr (KIND == MI_KV_INT8) {
+                const float scale = h_f(scales[cache]);
+                const u32x2 w = *reinterpret_cast<const u32x2*>(pool + cache * D + at);
                 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = static_cast<_Float16>(static_cast<float>(static_cast<int8_t>(w[e / 4] >> (8 * (e % 4)))) * scale);
+                for (int z = 0; z < 8; ++z)
+                    x[z] = static_cast<_Float16>(static_cast<float>(static_cast<int8_t>(w[z / 4] >> (8 * (z % 4)))) * scale);
             } else {
-                const float scale = h_f(scales[p.cache * (D / 32) + p.at / 32]);
-                const uint32_t w = *reinterpret_cast<const uint32_t*>(pool + (p.cache * D + p.at) / 2);
+                const float scale = h_f(scales[cache * (D / 32) + at / 32]);
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(pool + (cache * D + at) / 2);
                 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = static_cast<_Float16>(static_cast<float>(static_cast<int>(w >> (4 * e) & 15) - 8) * scale);
+                for (int z = 0; z < 8; ++z) x[z] = static_cast<_Float16>(static_cast<float>(static_cast<int>(w >> (4 * z) & 15) - 8) * scale);
             }
         }
+        if (wide) *reinterpret_cast<half8*>(dst + e) = x;
+        else
+            #pragma unroll
+            for (int z = 0; z < 8; ++z) dst[e + z] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[z]));
     }
-    uint16_t* dst = blockIdx.y ? v + p.row * ld_v : k + p.row * ld_k;
-    dst += p.head * D + p.at;
-    if (reinterpret_cast<uintptr_t>(dst) % 16 == 0) *reinterpret_cast<half8*>(dst) = x;
-    else
-        #pragma unroll
-        for (int e = 0; e < 8; ++e) dst[e] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x[e]));
 }
 
-// Blocks for one thread per 8 values of a row of keys; 0: more than a grid counts.
-unsigned blocks_for(const PagedArgs& a, int D) {
-    const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.n_kv_heads, per_block = kThreads / (D / kPiece);
-    const int64_t blocks = (rows + per_block - 1) / per_block;
-    return blocks > 0x7fffffff / kThreads ? 0u : static_cast<unsigned>(blocks);
+// Blocks for one wavefront per row of keys; 0 (and said): more than a grid counts.
+unsigned blocks_for(const char* who, const PagedArgs& a) {
+    const int64_t blocks = (a.n_tokens + static_cast<int64_t>(kThreads / 64) - 1) / (kThreads / 64);
+    if (blocks <= 0x7fffffff / kThreads) return static_cast<unsigned>(blocks);
+    MI_ERROR_FMT("%s: %d rows are more than a launch counts", who, a.n_tokens);
+    return 0;
 }
 
 bool bad_rows(const char* who, const void* k, int ld_k, const void* v, int ld_v, const PagedArgs& a, int D) {
@@ -240,11 +263,8 @@ extern "C" int mi_kv_write(void* stream, const mi_kv_cache* cache, const mi_kv_b
     PagedArgs a;
     if (!paged_args("mi_kv_write", cache, batch, &a) || bad_rows("mi_kv_write", k, ld_k, v, ld_v, a, cache->head_dim)) return 0;
     if (a.n_seqs == 0 || a.n_tokens == 0) return 1;
-    const unsigned blocks = blocks_for(a, cache->head_dim);
-    if (!blocks) {
-        MI_ERROR_FMT("mi_kv_write: %d rows of %d heads are more than a launch counts", a.n_tokens, a.n_kv_heads);
-        return 0;
-    }
+    const unsigned blocks = blocks_for("mi_kv_write", a);
+    if (!blocks) return 0;
     if (!ensure_init()) return 0;
     return MI_KV_LAUNCH(kv_write_kernel, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v));
 }
@@ -253,11 +273,8 @@ extern "C" int mi_kv_read(void* stream, const mi_kv_cache* cache, const mi_kv_ba
     PagedArgs a;
     if (!paged_args("mi_kv_read", cache, batch, &a) || bad_rows("mi_kv_read", k, ld_k, v, ld_v, a, cache->head_dim)) return 0;
     if (a.n_seqs == 0 || a.n_tokens == 0) return 1;
-    const unsigned blocks = blocks_for(a, cache->head_dim);
-    if (!blocks) {
-        MI_ERROR_FMT("mi_kv_read: %d rows of %d heads are more than a launch counts", a.n_tokens, a.n_kv_heads);
-        return 0;
-    }
+    const unsigned blocks = blocks_for("mi_kv_read", a);
+    if (!blocks) return 0;
     if (!ensure_init()) return 0;
     return MI_KV_LAUNCH(kv_read_kernel, static_cast<uint16_t*>(k), static_cast<uint16_t*>(v));
 }
