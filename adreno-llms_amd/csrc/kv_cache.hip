@@ -4,12 +4,13 @@
 //
 // scale = fp16(greatest |x| / top) with top = 127 or 7, code = x / scale to the nearest integer, ties to even.  Both are
 // exact: an fp16 number over 127 or 7 is never within 2^-9 of an fp16 step of the middle between two fp16 numbers, and a quotient of
-// two fp16 numbers that is not a half-integer is at least 2^-12 away from one, more than the fp32 division's error at 127.
+// two fp16 numbers that is not a half-integer is at least 2^-12 away from one, more than an fp32 quotient's error at 127.
 #include "../../include/mi_linear.h"
 #include "device_math.h"
 #include "paged.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace mi {
 namespace {
@@ -54,11 +55,15 @@ __device__ __forceinline__ Place place_of(const PagedArgs& a, int row) {
 
 // The greatest of the values of N neighbouring lanes (N = 4, 8, 16: a piece of a DPP row), in each of them.
 template <int N>
-__device__ __forceinline__ float max_of(float m) {
-    m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xb1, 0xf, 0xf, true)));     // lane ^ 1
-    m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4e, 0xf, 0xf, true)));     // lane ^ 2
-    if constexpr (N >= 8) m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x141, 0xf, 0xf, true)));  // half row mirrored
-    if constexpr (N >= 16) m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x140, 0xf, 0xf, true))); // row mirrored
+__device__ __forceinline__ uint32_t max_of(uint32_t m) {
+    auto with = [&](auto ctrl) {
+        const uint32_t o = __builtin_amdgcn_update_dpp(0, m, decltype(ctrl)::value, 0xf, 0xf, true);
+        m = o > m ? o : m;
+    };
+    with(std::integral_constant<int, 0xb1>{});                                 // lane ^ 1
+    with(std::integral_constant<int, 0x4e>{});                                 // lane ^ 2
+    if constexpr (N >= 8) with(std::integral_constant<int, 0x141>{});          // half rows mirrored
+    if constexpr (N >= 16) with(std::integral_constant<int, 0x140>{});         // rows mirrored
     return m;
 }
 
@@ -98,36 +103,41 @@ __global__ __launch_bounds__(kThreads) void kv_write_kernel(const PagedArgs a, c
             } else {
                 constexpr bool kInt8 = KIND == MI_KV_INT8;
                 constexpr float kTop = kInt8 ? 127.0f : 7.0f, kMost = kInt8 ? 515.5f : 9352.0f;     // (code * scale stays below 65520)
-                // 0 for all finite values, else NaN: a NaN would be lost among maxima
-                float big = 0.0f, bad = 0.0f;
+                // The greatest |x| as fp16 bits, which ascend with the value, an infinity's and NaNs' behind all finite ones.
+                const u32x4 bits = __builtin_bit_cast(u32x4, x) & 0x7fff7fffu;
+                uint32_t most = 0;
                 #pragma unroll
-                for (int z = 0; z < 8; ++z) {
-                    const float f = static_cast<float>(x[z]);
-                    big = fmaxf(big, fabsf(f));
-                    bad += f * 0.0f;
+                for (int z = 0; z < 4; ++z) {
+                    most = bits[z] >> 16 > most ? bits[z] >> 16 : most;
+                    most = (bits[z] & 0xffffu) > most ? bits[z] & 0xffffu : most;
                 }
-                if (bad != 0.0f) big = __builtin_huge_valf();
-                big = max_of<kInt8 ? D / kPiece : 32 / kPiece>(big);
-                const bool finite = big <= 65504.0f;
+                most = max_of<kInt8 ? D / kPiece : 32 / kPiece>(most);
+                const bool finite = most < 0x7c00u;
+                const float big = h_f(static_cast<uint16_t>(most));
                 const _Float16 h = static_cast<_Float16>(finite ? fminf(__fdiv_rn(big, kTop), kMost) : __builtin_nanf(""));
                 const float scale = static_cast<float>(h);
-                int code[8];
+                // x / scale from the reciprocal and what is left of x behind it (exact in fma): a half-integer comes out as such.
+                // (scale 0: reciprocal 0, all codes 0.)  Added to 1.5 * 2^23 the quotient is rounded to an integer, which is then in
+                // the low bits (Q4: plus 8).
+                const float inverse = finite && scale > 0.0f ? __builtin_amdgcn_rcpf(scale) : 0.0f, by = finite ? scale : 0.0f;
+                constexpr float kBase = 12582912.0f + (kInt8 ? 0.0f : 8.0f);
+                uint32_t code[8];
                 #pragma unroll
                 for (int z = 0; z < 8; ++z) {
-                    const float c = finite && scale > 0.0f ? rintf(__fdiv_rn(static_cast<float>(x[z]), scale)) : 0.0f;
-                    code[z] = static_cast<int>(fminf(fmaxf(c, kInt8 ? -127.0f : -8.0f), kTop));
+                    const float f = finite ? static_cast<float>(x[z]) : 0.0f, q = f * inverse;
+                    const float c = __builtin_amdgcn_fmed3f(fmaf(fmaf(-q, by, f), inverse, q), kInt8 ? -127.0f : -8.0f, kTop);
+                    code[z] = __float_as_uint(c + kBase);
                 }
+                // the low bytes of four
+                auto bytes = [&](int z, int step) {
+                    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(code[z + 3 * step], code[z + 2 * step], 0x0c0c0400u),
+                                                 __builtin_amdgcn_perm(code[z + step], code[z], 0x0c0c0400u), 0x05040100u);
+                };
                 if constexpr (kInt8) {
-                    u32x2 w = {0, 0};
-                    #pragma unroll
-                    for (int z = 0; z < 8; ++z) w[z / 4] |= static_cast<uint32_t>(code[z] & 255) << (8 * (z % 4));
-                    *reinterpret_cast<u32x2*>(pool + cache * D + at) = w;
+                    *reinterpret_cast<u32x2*>(pool + cache * D + at) = u32x2{bytes(0, 1), bytes(4, 1)};
                     if (at == 0) scales[cache] = __builtin_bit_cast(uint16_t, h);
                 } else {
-                    uint32_t w = 0;
-                    #pragma unroll
-                    for (int z = 0; z < 8; ++z) w |= static_cast<uint32_t>(code[z] + 8) << (4 * z);
-                    *reinterpret_cast<uint32_t*>(pool + (cache * D + at) / 2) = w;
+                    *reinterpret_cast<uint32_t*>(pool + (cache * D + at) / 2) = bytes(0, 2) | bytes(1, 2) << 4;
                     if (at % 32 == 0) scales[cache * (D / 32) + at / 32] = __builtin_bit_cast(uint16_t, h);
                 }
             }
