@@ -700,10 +700,10 @@ __device__ __forceinline__ void row_by_itself(const AttentionArgs& a, const int*
                 float dot = 0.0f;
                 #pragma unroll 1
                 for (int e = 0; e < D; ++e) dot = fmaf(h_f(q[e]), element<KIND, D>(a.p.k, a.p.k_scale, at, e), dot);
-                score = dot * a.scale * 1.44269504088896341f - kHead;
+                score = dot * a.scale * 1.44269504088896341f;
             }
         }
-        const float now = fmaxf(base, wave_max(score)), was = __builtin_amdgcn_exp2f(base - now);
+        const float now = fmaxf(base, wave_max(score) - kHead), was = __builtin_amdgcn_exp2f(base - now);
         const float w = hi < 0 ? 0.0f : static_cast<float>(static_cast<_Float16>(__builtin_amdgcn_exp2f(score - now)));
         base = now;
         sum *= was;
@@ -1113,12 +1113,19 @@ Plan make_plan(const AttentionArgs& a, int rows_per_set, int from, int to, int w
     return plan;
 }
 
+bool fits_a_grid(int64_t blocks, int threads) {
+    if (blocks <= 0xffffffffll / threads) return true;
+    MI_ERROR_FMT("mi_attention: %lld blocks are more than a launch counts", static_cast<long long>(blocks));
+    return false;
+}
+
 template <int KIND, int D>
 bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to) {
     int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (slot_floats(D) * sizeof(float))) : 0, blocks = 0;
     if (slots > kSliceCounters) slots = kSliceCounters;
     Plan plan = make_plan(a, kRows, 0, to, 3 * device_info().cus, slots, &blocks);
     plan.least = 16;
+    if (!fits_a_grid(blocks, 64 * kWaves)) return false;
     auto go = [&](auto kern) {
         hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, a, plan, static_cast<float*>(workspace),
                            workspace ? slice_counters(workspace) : nullptr);
@@ -1157,6 +1164,7 @@ bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int fr
     const int64_t want = two ? (sets < cus ? cus - sets : 0) : 2 * cus;
     Plan plan = make_plan(a, kChunkRows, from, 0x7fffffff, static_cast<int>(want), slots, &blocks);
     plan.least = 4;
+    if (!fits_a_grid(blocks, 64 * kChunkWaves * 2)) return false;
     return two ? launch_slices<KIND, D, 2>(s, a, plan, blocks, workspace) : launch_slices<KIND, D, 1>(s, a, plan, blocks, workspace);
 }
 

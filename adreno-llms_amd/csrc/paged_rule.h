@@ -41,17 +41,6 @@ constexpr Span span_of(int start, int end, int len, int n_tokens) {
     return s;
 }
 
-// The sequence that row r belongs to: the last one that starts at or before it (-1: none).
-constexpr int sequence_of(const int* q_start, int n_seqs, int r) {
-    int lo = 0, hi = n_seqs;                       // q_start[lo - 1] <= r < q_start[hi], as far as they ascend
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (q_start[mid] <= r) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo - 1;
-}
-
 // Positions that a table of max_pages pages has, as far as an int counts them.
 constexpr int capacity(int max_pages, int page_size) {
     const long long c = static_cast<long long>(max_pages) * page_size;

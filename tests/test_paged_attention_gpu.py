@@ -84,6 +84,20 @@ def test_what_a_masked_position_holds_does_not_matter(queue, kind, form):
         assert np.isnan(got[n - 3]).any() and np.isnan(got[n - 5]).any()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv_heads,D,m,n", [(14, 2, 64, 1500, 400), (14, 2, 64, 1300, 1300), (8, 2, 128, 900, 300)])
+def test_the_same_where_a_sequence_is_taken_in_parts(queue, kind, heads, kv_heads, D, m, n):
+    c = Cache(kind, heads, kv_heads, D, 16, [m, 40], [n, 1], seed=21)
+    for p, bad in ((m - 7, np.inf), (m - 150, np.nan)):
+        c.v[0][p, kv_heads - 1, 3] = bad
+    c.fill()
+    got = c.upload().attend(queue)
+    c.check(got, rows=np.r_[0:n - 150, n])
+    group = heads // kv_heads
+    assert np.isnan(got[n - 150:n, (kv_heads - 1) * group:, 3]).all()
+    assert np.isfinite(got[:n, :(kv_heads - 1) * group]).all() and np.isfinite(got[n - 150:n, :, 4] if kind == mil.KV_F16 else 0).all()
+
+
 def test_infinite_values_that_are_seen(queue):
     c = Cache(mil.KV_F16, 14, 2, 64, 16, [40], [40], seed=7)
     c.v[0][20, 1, 3], c.v[0][25, 1, 3] = np.inf, -np.inf
@@ -200,3 +214,131 @@ def test_steps_of_a_recorded_graph(queue, kind):
             part.k, part.v = [k[:p + 1] for k, p in zip(c.k, now)], [v[:p + 1] for v, p in zip(c.v, now)]
             part.qkv[:] = rows
             part.check(out.read(np.float16, (3, c.heads, c.D)), what=t)
+
+
+@pytest.mark.parametrize("kind,heads,kv_heads,D,page,m,n", [
+    (mil.KV_F16, 32, 8, 128, 64, 2000, 2000), (mil.KV_INT8, 14, 2, 64, 16, 1400, 1300), (mil.KV_Q4, 16, 8, 64, 100, 2100, 700),
+    (mil.KV_F16, 8, 1, 128, 128, 9000, 40), (mil.KV_F16, 14, 2, 64, 16, 20000, 3)])
+def test_long_ones(queue, kind, heads, kv_heads, D, page, m, n):
+    """Every way that blocks share a long prompt, a chunk far in, and a few tokens behind many."""
+    c = Cache(kind, heads, kv_heads, D, page, [m], [n], seed=22).upload()
+    c.check(c.attend(queue))
+    c.check(c.attend(queue, window=777, sinks=5), window=777, sinks=5)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 70])
+def test_one_key_outweighs_thousands(queue, kind, n):
+    """Weights down to 2^-22 of the greatest, of which there are enough to count for a hundredth."""
+    c = Cache(kind, 14, 2, 64, 32, [9000], [n], seed=23)
+    unit = np.ones(64) / 8
+    c.qkv[:, :14 * 64] = np.tile(unit * 8, 14).astype(np.float16)           # q k = 8 per unit of k: scores 15.2 and 0
+    c.k[0][:] = 0
+    c.k[0][17] = (unit * 15.2).astype(np.float16)
+    c.v[0][:] = np.abs(c.v[0])
+    c.fill()
+    c.upload()
+    c.check(c.attend(queue))
+
+
+def test_pools_beyond_4_gib(queue):
+    """Pages at offsets that 32 bits do not hold."""
+    page, kv, D, n_pages = 64, 8, 128, 36000
+    small = Cache(mil.KV_F16, 16, kv, D, page, [300, 64], [1, 30], seed=24)
+    size = kv * page * D * 2
+    assert n_pages * size > 2 ** 32
+    far = np.full_like(small.table, -1)
+    used = [(b, i) for b in range(2) for i in range(small.max_pages) if small.table[b, i] >= 0]
+    places = [n_pages - 1, 16384, 16383, 1, 35001, 32769, 20000][:len(used)]
+    pools = [mil.Buffer(n_pages * size) for _ in "kv"]
+    for (b, i), to in zip(used, places):
+        far[b, i] = to
+        for pool, name in zip(pools, "kv"):
+            host = np.ascontiguousarray(small.pool[name][small.table[b, i]])
+            assert mil.lib().mi_memcpy_h2d(pool.ptr + to * size, host.ctypes.data, size, None)
+    small.upload()
+    small.dev_table.write(far)
+    small.cache = mil.KVCache(mil.KV_F16, n_pages, page, kv, D, *pools)
+    small.check(small.attend(queue))
+    # the new rows read back from there, and written there again
+    outs = [mil.Buffer(small.rows * kv * D * 2) for _ in "kv"]
+    assert mil.kv_read(queue, small.cache, small.batch, *outs)
+    at = small.dev_qkv.ptr + 2 * small.heads * D
+    assert mil.kv_write(queue, small.cache, small.batch, at, at + 2 * kv * D, small.ld, small.ld)
+    queue.finish()
+    for out, each in zip(outs, (small.k, small.v)):
+        new = np.concatenate([x[m - n:] for x, m, n in zip(each, small.lengths, small.new)]).reshape(small.rows, -1)
+        assert np.array_equal(out.read(np.uint16, new.shape), new.view(np.uint16))
+    small.check(small.attend(queue))
+
+
+def test_sequences_that_share_pages(queue):
+    """A prompt that two answers go on from: the same pages in both tables."""
+    c = Cache(mil.KV_INT8, 14, 2, 64, 16, [70, 70], [1, 1], seed=25)
+    for each in (c.k, c.v):
+        each[1][:64] = each[0][:64]
+    c.fill()
+    c.table[1, :4] = c.table[0, :4]
+    c.upload()
+    c.check(c.attend(queue))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_layer_of_a_batch(queue, kind):
+    """What a host does for a decoder layer of several conversations: q | k | v in one product with stacked int8 weights, the
+    new rows into their pages, attention, and the output projection, twice over from a recorded graph, with the lengths going up."""
+    heads, kv, D, hidden, page = 14, 2, 64, 896, 16
+    lengths, new = [150, 3, 61], [4, 1, 1]
+    c = Cache(kind, heads, kv, D, page, lengths, new, seed=26)
+    rows, width = sum(new), heads * D
+    keep = []
+
+    def weight(seed, n, k):
+        w = mil.synth_normal_f16(seed, 0.02, (n, k))
+        q, s = mil.quantize_int8(w)
+        keep.extend([mil.Buffer.from_host(q), mil.Buffer.from_host(s)])
+        assert mil.nnopt_register_int8_weight(keep[-2], keep[-1], n, k)
+        return keep[-2], (q.astype(np.float64) * s.astype(np.float64)[:, None])
+
+    wqkv, full_qkv = weight(1, c.ld, hidden)
+    wo, full_o = weight(2, hidden, width)
+    c.upload()
+    x = [mil.synth_normal_f16(10 + t, 1.0, (rows, hidden)) for t in range(2)]
+    xb, att, out = mil.Buffer(rows * hidden * 2), mil.Buffer(rows * width * 2), mil.Buffer(rows * hidden * 2)
+    at = c.dev_qkv.ptr + 2 * width
+    call = mil.AttentionCall(c.cache, c.batch, heads, c.dev_qkv, att, ld_q=c.ld)
+
+    def layer():
+        assert mil.pytorch_linear(queue, rows, c.ld, hidden, xb, wqkv, c.dev_qkv)
+        assert mil.kv_write(queue, c.cache, c.batch, at, at + 2 * kv * D, c.ld, c.ld)
+        assert mil.attention(queue, call)
+        assert mil.pytorch_linear(queue, rows, hidden, width, att, wo, out)
+
+    xb.write(x[0])
+    layer()                                              # the first use of the kernels, outside the recording
+    queue.finish()
+    with mil.Graph(queue) as graph:
+        layer()
+    for t in range(2):
+        step = [m + t * n for m, n in zip(lengths, new)]
+        c.dev_len.write(np.array(step, np.int32))
+        xb.write(x[t])
+        graph.launch()
+        queue.finish()
+        qkv = c.dev_qkv.read(np.float16, (rows, c.ld))
+        assert np.abs(qkv.astype(np.float64) - x[t].astype(np.float64) @ full_qkv.T).max() < 2e-2       # (fp16 of values up to 4)
+        # the cache as it has to be now
+        if t == 0:
+            c.k, c.v = [k[:m - n] for k, m, n in zip(c.k, lengths, new)], [v[:m - n] for v, m, n in zip(c.v, lengths, new)]
+        part = Cache(kind, heads, kv, D, page, step, new)
+        kv_rows = qkv[:, width:].reshape(rows, 2, kv, D)
+        for b, (s, n) in enumerate(zip(c.start, new)):
+            c.k[b] = np.concatenate([c.k[b], kv_rows[s:s + n, 0]])
+            c.v[b] = np.concatenate([c.v[b], kv_rows[s:s + n, 1]])
+        part.k, part.v, part.qkv = c.k, c.v, qkv
+        got = att.read(np.float16, (rows, heads, D))
+        part.check(got, what=t)
+        want = got.reshape(rows, width).astype(np.float64) @ full_o.T
+        assert np.abs(out.read(np.float16, (rows, hidden)).astype(np.float64) - want).max() < 2e-2
+    for w in (wqkv, wo):
+        mil.nnopt_unregister_weight(w)

@@ -15,7 +15,6 @@ DRIVER = """
 using namespace mi;
 extern "C" int quotient(int n, int d) { return divide(n, make_divider(d)); }
 extern "C" void span(int s, int e, int len, int rows, int* out) { const Span x = span_of(s, e, len, rows); out[0] = x.first; out[1] = x.n; out[2] = x.pos; }
-extern "C" int sequence(const int* q, int n, int r) { return sequence_of(q, n, r); }
 extern "C" int cap_of(int pages, int size) { return capacity(pages, size); }
 extern "C" int seen(int p, int j, int w, int s) { return sees(p, j, w, s); }
 extern "C" int every(int j0, int size, int lo, int hi, int cap, int w, int s) { return all_seen(j0, size, lo, hi, cap, w, s); }
@@ -60,14 +59,6 @@ def test_rows_of_a_sequence(rule):
                 assert 0 <= first <= 10 and 0 <= n <= 10 - first and pos == max(length, 0) - n
                 if 0 <= s <= e <= 10:
                     assert (first, n) == (s, e - s)
-    starts = [0, 0, 3, 3, 3, 9, 9]
-    q = (ctypes.c_int * len(starts))(*starts)
-    for r in range(12):
-        b = rule.sequence(q, 6, r)
-        want = max(i for i in range(7) if starts[i] <= r)
-        assert b == min(want, 5)
-    q = (ctypes.c_int * 3)(4, 9, 9)
-    assert rule.sequence(q, 2, 3) == -1 and rule.sequence(q, 0, 3) == -1
     assert rule.cap_of(3, 16) == 48 and rule.cap_of(BIG, BIG) == BIG
 
 
