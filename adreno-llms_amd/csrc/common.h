@@ -189,6 +189,10 @@ constexpr int kSliceCounters = 16384;
 inline uint32_t* slice_counters(void* workspace) {
     return reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kWorkspaceBytes);
 }
+// Behind the counters: room for the sums of attention's rows whose keys several blocks share (paged_attention.hip).
+constexpr size_t kPartialBytes = 32u << 20;
+inline float* attention_sums(void* workspace) { return reinterpret_cast<float*>(slice_counters(workspace) + kSliceCounters); }
+constexpr size_t kAllWorkspaceBytes = kWorkspaceBytes + kSliceCounters * sizeof(uint32_t) + kPartialBytes;
 // runtime.hip: the same for a registered W where mi_linear would run the GEMM
 int linear_glu(hipStream_t s, int M, int N, int K, const void* x, const void* W, void* out);
 // gemm.hip, runtime.hip: the sums of the K slices of a GEMM that mi_linear would cut into slices, left in the stream's

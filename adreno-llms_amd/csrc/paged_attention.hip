@@ -660,20 +660,27 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kern
 
 // ---- many rows: tiles of keys in LDS, 32 rows per wavefront -------------------------------------------------
 //
-// A block has 128 rows of one sequence and key/value head, 32 per wavefront (v_mfma_f32_32x32x16_f16: twice the rows per
+// A block has 128 or 64 rows of one sequence and key/value head, 32 per wavefront (v_mfma_f32_32x32x16_f16: twice the rows per
 // operand that comes out of LDS), and takes its tiles of 64 keys through two buffers in LDS: while a tile is multiplied the next one
-// is on its way to registers, and is written (int8 and Q4: as fp16, converted once for the block) behind it.
+// is on its way to registers, and is written (int8 and Q4: as fp16, converted once for the block) behind it.  KS slices of a block
+// take every KS-th tile, each with buffers of its own.
 // Scores again transposed: lane (query = lane % 32, half h = lane / 32) has keys 8 a + 4 h + b of every 32, a, b = 0 .. 3, in
 // registers 4 a + b, and registers 8 c .. 8 c + 7 are the B operand of the product with the values for keys 16 c + 4 h .. and 16 c + 8 +
 // 4 h ..  The A operand, 4 keys of one element at a time, is what a transposed read from LDS gives.
 // In a row of LDS the 16-byte piece p lies at p ^ twist(row): eight rows' pieces of one p, and four rows' two neighbouring pieces,
 // are in different banks.
+//
+// What bounds it: a wavefront alone takes 1.3 us per tile at width 64, of which the matrix cores are busy 0.25 and the vector units
+// (exponentials, maxima, conversions) 0.4; the rest is the chain barrier - keys from LDS - scores - weights - values - next tile to LDS, which
+// only other wavefronts fill: matrix cores busy 22 % of the SIMD-cycles, vector units 30 %, LDS 34 % of the CU-cycles (a third of it
+// bank conflicts) at 4096 rows of 32 heads over 8, width 128, window 1000 (0.55 PFLOP/s).  Tried and slower: the next tile's
+// scores under this one's weights (32 or more registers), the next tile to LDS while scores are formed, all key operands read ahead.
 
-constexpr int kChunkKeys = 64, kChunkWaves = 4, kChunkRows = 32 * kChunkWaves;
-constexpr int chunk_slot_floats(int D) { return kChunkRows * (D + 2); }
+constexpr int kChunkKeys = 64;
+constexpr int chunk_slot_floats(int D, int RW) { return 32 * RW * (D + 2); }
 constexpr int chunk_lds(int D) { return 2 * 2 * kChunkKeys * 2 * D; }          // of a slice's tiles
 constexpr int chunk_lds_all(int D, int KS) { return KS * (chunk_lds(D) + 2 * kChunkKeys); }
-constexpr int meet_bytes(int D) { return kChunkWaves * 64 * (D / 2 + 3) * 4; }    // of a slice's sums
+constexpr int meet_floats(int D, int RW) { return RW * 64 * (D / 2 + 3); }         // of a slice's sums
 __device__ __forceinline__ constexpr int twist(int row) { return (row & 3) * 2 + (row >> 2 & 1); }
 
 // Row `q` (fp16) of a query at position pos against tiles first .. last - 1 of a sequence, one key to a lane: where an infinity or a
@@ -720,9 +727,10 @@ __device__ __forceinline__ void row_by_itself(const AttentionArgs& a, const int*
     }
 }
 
-template <int KIND, int D, bool PAGES16, int KS>
-__global__ __launch_bounds__(64 * kChunkWaves * KS, 2) void paged_chunk_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ partial,
+template <int KIND, int D, bool PAGES16, int RW, int KS>
+__global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ partial,
                                                                           uint32_t* __restrict__ counters) {
+    constexpr int kChunkWaves = RW, kChunkRows = 32 * RW;
     constexpr int kRow = row_bytes(KIND, D), kScales = row_scales(KIND, D);
     constexpr int kPiece = KIND == MI_KV_Q4 && D == 64 ? 8 : 16, kPieces = kRow / kPiece;      // of a row as it is stored
     constexpr int kPer = 64 * kChunkWaves / kPieces;                                           // rows that the block loads at a time
@@ -980,32 +988,38 @@ __global__ __launch_bounds__(64 * kChunkWaves * KS, 2) void paged_chunk_kernel(c
             if (busy && j0 <= p_hi && (j0 + kChunkKeys > w_first || j0 < sinks)) multiply(v, buf);
         }
     }
-    if constexpr (KS == 2) {
-        // The second slice's sums come to the first by LDS.
+    if constexpr (KS > 1) {
+        // The other slices' sums come to the first by LDS, in their order.
         __syncthreads();
+        constexpr int kBox = meet_floats(D, RW);
         float* const box = reinterpret_cast<float*>(lds) + wave * 64 * (D / 2 + 3) + lane;
-        if (slice == 1) {
-            box[0] = base;
-            box[64] = sum;
-            box[128] = odd ? 1.0f : 0.0f;
+        if (slice > 0) {
+            float* const to = box + (slice - 1) * kBox;
+            to[0] = base;
+            to[64] = sum;
+            to[128] = odd ? 1.0f : 0.0f;
             #pragma unroll
             for (int m = 0; m < kOuts; ++m)
                 #pragma unroll
-                for (int r = 0; r < 16; ++r) box[(3 + 16 * m + r) * 64] = acc[m][r];
+                for (int r = 0; r < 16; ++r) to[(3 + 16 * m + r) * 64] = acc[m][r];
         }
         __syncthreads();
-        if (slice == 1) return;
-        const float now = fmaxf(base, box[0]), was = __builtin_amdgcn_exp2f(base - now), f = __builtin_amdgcn_exp2f(box[0] - now);
-        base = now;
-        sum = sum * was + box[64] * f;
-        odd |= __any(box[128] != 0.0f) != 0;
+        if (slice > 0) return;
         #pragma unroll
-        for (int m = 0; m < kOuts; ++m)
+        for (int z = 0; z < KS - 1; ++z) {
+            const float* const from = box + z * kBox;
+            const float now = fmaxf(base, from[0]), was = __builtin_amdgcn_exp2f(base - now), f = __builtin_amdgcn_exp2f(from[0] - now);
+            base = now;
+            sum = sum * was + from[64] * f;
+            odd |= __any(from[128] != 0.0f) != 0;
             #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[m][r] = acc[m][r] * was + box[(3 + 16 * m + r) * 64] * f;
+            for (int m = 0; m < kOuts; ++m)
+                #pragma unroll
+                for (int r = 0; r < 16; ++r) acc[m][r] = acc[m][r] * was + from[(3 + 16 * m + r) * 64] * f;
+        }
     }
     if (!busy) return;
-    constexpr int kSlot = chunk_slot_floats(D) / 2, kPairs = kOuts * 8;           // pairs of floats: of a block, of a lane
+    constexpr int kSlot = chunk_slot_floats(D, RW) / 2, kPairs = kOuts * 8;           // pairs of floats: of a block, of a lane
     auto* const all = reinterpret_cast<uint64_t*>(partial);
     const int64_t own = static_cast<int64_t>(blockIdx.x) * kSlot;
     const int at = wave * kPairs * 64 + lane, at_sum = kChunkWaves * kPairs * 64 + wave * 32 + i;
@@ -1121,13 +1135,13 @@ bool fits_a_grid(int64_t blocks, int threads) {
 
 template <int KIND, int D>
 bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to) {
-    int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (slot_floats(D) * sizeof(float))) : 0, blocks = 0;
+    int64_t slots = workspace ? static_cast<int64_t>(kPartialBytes / (slot_floats(D) * sizeof(float))) : 0, blocks = 0;
     if (slots > kSliceCounters) slots = kSliceCounters;
     Plan plan = make_plan(a, kRows, 0, to, 3 * device_info().cus, slots, &blocks);
     plan.least = 16;
     if (!fits_a_grid(blocks, 64 * kWaves)) return false;
     auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, a, plan, static_cast<float*>(workspace),
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, a, plan, workspace ? attention_sums(workspace) : nullptr,
                            workspace ? slice_counters(workspace) : nullptr);
     };
     if (a.p.page.d % 16 == 0) go(paged_step_kernel<KIND, D, true>);
@@ -1135,37 +1149,43 @@ bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to)
     return MI_HIP_OK(hipGetLastError());
 }
 
-template <int KIND, int D, int KS>
-bool launch_slices(hipStream_t s, const AttentionArgs& a, const Plan& plan, int64_t blocks, void* workspace) {
-    constexpr int lds = chunk_lds_all(D, KS);
-    static_assert(lds <= 160 * 1024 && (KS == 1 || meet_bytes(D) <= KS * chunk_lds(D)), "tiles and sums fit");
+template <int KIND, int D, int RW, int KS>
+bool launch_slices(hipStream_t s, const AttentionArgs& a, void* workspace, int from, int64_t want) {
+    constexpr int lds = chunk_lds_all(D, KS), threads = 64 * RW * KS;
+    static_assert(lds <= 160 * 1024 && (KS - 1) * meet_floats(D, RW) * 4 <= KS * chunk_lds(D), "tiles and sums fit");
+    int64_t slots = workspace ? static_cast<int64_t>(kPartialBytes / (chunk_slot_floats(D, RW) * sizeof(float))) : 0, blocks = 0;
+    if (slots > kSliceCounters / RW) slots = kSliceCounters / RW;
+    Plan plan = make_plan(a, 32 * RW, from, 0x7fffffff, static_cast<int>(want), slots, &blocks);
+    plan.least = 4;
+    if (!fits_a_grid(blocks, threads)) return false;
     auto go = [&](auto kern) {
         if (lds > 65536 && !MI_ONCE_OK(MI_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))))
             return false;
-        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kChunkWaves * KS), lds, s, a, plan, static_cast<float*>(workspace),
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(threads), lds, s, a, plan, workspace ? attention_sums(workspace) : nullptr,
                            workspace ? slice_counters(workspace) : nullptr);
         return MI_HIP_OK(hipGetLastError());
     };
-    return a.p.page.d % 16 == 0 ? go(paged_chunk_kernel<KIND, D, true, KS>) : go(paged_chunk_kernel<KIND, D, false, KS>);
+    return a.p.page.d % 16 == 0 ? go(paged_chunk_kernel<KIND, D, true, RW, KS>) : go(paged_chunk_kernel<KIND, D, false, RW, KS>);
 }
 
 template <int KIND, int D>
 bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int from) {
-    int64_t slots = workspace ? static_cast<int64_t>(kWorkspaceBytes / (chunk_slot_floats(D) * sizeof(float))) : 0, blocks = 0;
-    if (slots > kSliceCounters / kChunkWaves) slots = kSliceCounters / kChunkWaves;
     int64_t sets = 0;
-    (void)make_plan(a, kChunkRows, from, 0x7fffffff, 0, 0, &sets);
-    // A block of eight wavefronts, two slices of a set's keys, is alone on its CU; of four wavefronts there are two.  So few sets
-    // are taken in two slices (us with / without: 300 rows of 14 heads at 900 int8 15.0 / 15.3, width 128 in 17 conversations, 208 sets,
-    // 100 / 125) and many are not (2048 rows of 14 heads, 224 sets, 33.7 / 29.7: a second round); wide heads, where a wavefront's tile takes
-    // twice as long, up to more of them.  Parts of sets meet in memory as well, as many as blocks are resident.
+    (void)make_plan(a, 128, from, 0x7fffffff, 0, 0, &sets);
     const int64_t cus = device_info().cus;
+    // A set's tiles are one chain of about 1.3 us each (width 128: twice that), so where there are few sets several wavefronts take them
+    // in turn.  A block of eight wavefronts is alone on its CU, of four wavefronts two are resident; sums of slices meet in LDS,
+    // of parts in memory, 33 KB per block.  Measured, us, width 64, at 128 rows / 128 in two slices / 64 in four slices:
+    //   2048 rows of 14 heads over 2 (224 sets) 28.5 / 33.7 / 33.5: blocks enough; 300 at 900, int8, 15.3 / 15.0 / 14.5; 676 of 16 over 8 in
+    //   a window of 435 (88 sets) 19.4 / 16.8 / 14.9; 14 sequences of 9 over 3 in a window of 137 21.4 / 18.6 / 16.6; 64 rows of 71, two
+    //   tiles, 8.6 / 8.0 / 8.8.
+    // Width 128, 128 rows / in two slices: 17 conversations of 32 heads over 8 (208 sets) 125 / 100, 14 of 16 over 8 90 / 74; 1024 sets 109 / -.
+    if constexpr (D == 64)
+        if (sets <= cus / 2 && a.p.cap > 4 * kChunkKeys)
+            return launch_slices<KIND, D, 2, 4>(s, a, workspace, from, cus > 2 * sets ? cus - 2 * sets : 0);
     const bool two = sets <= (D == 128 ? cus * 3 / 2 : cus / 2);
     const int64_t want = two ? (sets < cus ? cus - sets : 0) : 2 * cus;
-    Plan plan = make_plan(a, kChunkRows, from, 0x7fffffff, static_cast<int>(want), slots, &blocks);
-    plan.least = 4;
-    if (!fits_a_grid(blocks, 64 * kChunkWaves * 2)) return false;
-    return two ? launch_slices<KIND, D, 2>(s, a, plan, blocks, workspace) : launch_slices<KIND, D, 1>(s, a, plan, blocks, workspace);
+    return two ? launch_slices<KIND, D, 4, 2>(s, a, workspace, from, want) : launch_slices<KIND, D, 4, 1>(s, a, workspace, from, want);
 }
 
 // Sequences of up to kFew rows run on the kernel for few rows, the others on the one for many; both run where the batch may

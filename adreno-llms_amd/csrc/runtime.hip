@@ -78,7 +78,7 @@ bool clear_counters(void* workspace) {
 
 void add_workspace(hipStream_t s) {
     void* p = nullptr;
-    if (hipMalloc(&p, kWorkspaceBytes + kSliceCounters * sizeof(uint32_t)) != hipSuccess || !clear_counters(p)) {
+    if (hipMalloc(&p, kAllWorkspaceBytes) != hipSuccess || !clear_counters(p)) {
         (void)hipGetLastError();      // no workspace: that stream's GEMMs run unsliced
         (void)hipFree(p);
         return;
