@@ -9,6 +9,7 @@
 #include "device_math.h"
 #include "paged.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace mi {
@@ -1188,13 +1189,29 @@ bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int fr
     return two ? launch_slices<KIND, D, 4, 2>(s, a, workspace, from, want) : launch_slices<KIND, D, 4, 1>(s, a, workspace, from, want);
 }
 
-// Sequences of up to kFew rows run on the kernel for few rows, the others on the one for many; both run where the batch may
-// have both (n_tokens and max_tokens do not say that all sequences have the same).
-constexpr int kFew = 32;
+// Which kernel.  The one for few rows reads the keys again for every 16 rows and has no start to pay for, the one for many
+// rows takes a tile for 64 or 128 and first fills its LDS: about 1.3 us per tile, 4 to 6 us before the first.  So what counts is
+// the work, in tiles of 16 rows by 32 keys: up to kEachCu per compute unit the whole batch is for the kernel for few rows, and
+// above that only its sequences of up to kFew rows.  Kernel for few rows / for many, us, fp16:
+//   14 heads over 2, width 64, 1 sequence: 112 sets of 16 rows at 1000 positions (14 tiles per compute unit) 8.9 / 12.4,
+//     224 (28) 11.9 / 13.6, 448 (55) 19.1 / 14.3; 28 at 16000 (55) 23.5 / 29.2, 56 (109) 35 / 25.4, 112 (219) 56 / 28.6.
+//   32 sequences: 448 sets at 500 (27) 9.9 / 11.5, 896 (55) 13.1 / 12.9, 1792 (110) 18.9 / 15.2;
+//     256 at 3000 (94) 19.8 / 20.1, 896 (328) 40 / 23.
+//   32 heads over 8, width 128, 1 sequence: 256 sets at 1000 (31) 16.4 / 22.8, 512 (62) 28.8 / 23.7; 64 at 16000 (125) 47.7 / 64.2, 128 (250) 79 / 55.
+//   16 heads of their own, width 128: 512 sets at 600 (38) 15.8 / 20.8, 1024 (76) 23.8 / 21.8.
+//   300 tokens of 14 heads behind 900, int8 12.8 / 14.0.
+//   Up to 32 rows, at any length: 8 sequences of 28 rows at 2000 8.6 / 13.1; 32 rows, width 128, at 2000 11.9 / 19.5.
+// The host knows the lengths' bound alone, the page table's width (or the window): a table much wider than its sequences are
+// long moves them to the kernel for many rows sooner.
+constexpr int kFew = 32, kEachCu = 48;
 template <int KIND, int D>
 bool launch(hipStream_t s, const AttentionArgs& a, void* workspace) {
     const int64_t most = static_cast<int64_t>(a.max_tokens) * (a.n_heads / a.p.n_kv_heads);
-    if (most <= kFew) return launch_step<KIND, D>(s, a, workspace, 0x7fffffff);
+    int64_t sets = 0, keys = a.p.cap;
+    (void)make_plan(a, kRows, 0, 0x7fffffff, 0, 0, &sets);
+    if (a.window > 0) keys = std::min(keys, static_cast<int64_t>(a.window) + a.sinks + a.max_tokens);
+    if (most <= kFew || sets * (keys / kKeys + 1) <= static_cast<int64_t>(kEachCu) * device_info().cus)
+        return launch_step<KIND, D>(s, a, workspace, 0x7fffffff);
     if (a.p.n_seqs == 1 || static_cast<int64_t>(a.max_tokens) * a.p.n_seqs == a.p.n_tokens) return launch_chunk<KIND, D>(s, a, workspace, 0);
     return launch_chunk<KIND, D>(s, a, workspace, kFew + 1) && launch_step<KIND, D>(s, a, workspace, kFew);
 }

@@ -43,6 +43,8 @@ class Cache:
     """Sequences of `lengths` positions whose last `new` are the batch's rows, in pages handed out in a random order.  What no
     sequence has written is NaN all over: pages of nobody, the rest of last pages, scales."""
 
+    columns = 0                                       # of the page table, in positions: at least that many (the tail is not used)
+
     def __init__(self, kind, heads, kv_heads, D, page, lengths, new, seed=0, pad=0, spare=3, max_pages=None, sigma=1.0, gap=0):
         rng = np.random.default_rng(seed)
         self.kind, self.heads, self.kv, self.D, self.page = kind, heads, kv_heads, D, page
@@ -51,7 +53,7 @@ class Cache:
         self.v = [(rng.standard_normal((n, kv_heads, D)) * sigma).astype(np.float16) for n in lengths]
         used = [-(-n // page) for n in lengths]
         self.n_pages = sum(used) + spare
-        self.max_pages = max_pages or max(max(used), 1)
+        self.max_pages = max_pages or max(max(used), 1, self.columns // page)
         order, at = rng.permutation(self.n_pages), 0
         self.table = np.full((len(lengths), self.max_pages), -1, np.int32)
         for b, n in enumerate(used):

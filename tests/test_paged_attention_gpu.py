@@ -16,6 +16,14 @@ def queue():
     return mil.Queue()
 
 
+@pytest.fixture(autouse=True, params=[0, 2 ** 20], ids=["tight", "wide"])
+def columns(request, monkeypatch):
+    """Small batches run on the kernel for few rows; under a page table for a million positions per sequence every sequence of more
+    than 32 rows runs on the one for many."""
+    monkeypatch.setattr(Cache, "columns", request.param)
+    return request.param
+
+
 STEPS = [
     dict(heads=14, kv_heads=2, D=64, page=16, lengths=[24], new=[1]),
     dict(heads=9, kv_heads=3, D=64, page=64, lengths=[1, 2, 31, 32, 33, 63, 64, 65, 500, 0], new=[1] * 9 + [0], pad=2),
@@ -49,6 +57,17 @@ def test_against_64_bits(queue, kind, case):
 @pytest.mark.parametrize("case", [STEPS[1], STEPS[4], CHUNKS[0], CHUNKS[2], CHUNKS[5]])
 @pytest.mark.parametrize("kind", [mil.KV_F16, mil.KV_Q4])
 def test_windows(queue, kind, case, window, sinks):
+    c = Cache(kind, seed=2, **case).upload()
+    c.check(c.attend(queue, window=window, sinks=sinks), window, sinks)
+
+
+@pytest.mark.parametrize("columns", [0], indirect=True)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (33, 0), (100, 37), (64, 64), (190, 1)])
+@pytest.mark.parametrize("case", [dict(heads=16, kv_heads=16, D=64, page=16, lengths=[200, 230] * 20, new=[200] * 40),
+                                  dict(heads=28, kv_heads=4, D=128, page=48, lengths=[210, 200, 399, 230] * 5, new=[200] * 20, pad=3)])
+@pytest.mark.parametrize("kind", [mil.KV_F16, mil.KV_Q4])
+def test_windows_of_many_rows(queue, kind, case, window, sinks):
+    """Enough rows for the kernel for many of them whatever the window."""
     c = Cache(kind, seed=2, **case).upload()
     c.check(c.attend(queue, window=window, sinks=sinks), window, sinks)
 
