@@ -26,9 +26,9 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kNone = -__builtin_huge_valf();  // the score of a key that the query does not see
 constexpr float kStart = -1.0e30f;               // the running maximum of a query that has seen no key
-// Weights are exp2(score - base) with base between 2^-7 and 2^8 .. below the greatest: between 2^7 and 2^15 for the greatest
-// score, so that fp16 holds weights down to 2^-21 of it at full precision, and the maximum may rise by 2^kSlack before the
-// sums are rescaled.
+// Weights are exp2(score - base).  base is set to kHead below the greatest score so far and stays until a score is more than kHead + kSlack
+// above it: so the greatest weight is between 2^7 and 2^15, fp16 holds weights down to 2^-21 of it at full precision, and the sums
+// are rescaled only where the maximum has risen by more than kSlack.
 constexpr float kHead = 7.0f, kSlack = 8.0f;
 
 // The greater of a lane's value and those of the lanes 16, 32 and 48 away.
@@ -328,6 +328,19 @@ __device__ __forceinline__ bool odd_values(const Tile<KIND, D, PAGES16>& t, cons
 }
 
 // ---- few rows: keys straight from memory to registers -----------------------------------------------------
+//
+// A block has 16 rows and a share of their tiles of 32 keys, which its four wavefronts take in turn, each with a maximum and sums of its
+// own that meet in LDS at the end.  No barrier in the loop, and no LDS: keys and values go from memory to the registers that are the
+// matrix instructions' operands, and as soon as a tile's keys are multiplied the next tile's are asked for into the same registers.
+// Blocks that share a set leave sums in the workspace; the last to arrive adds them in their order, so the bits are the same again.
+//
+// What bounds it: memory where the cache is long (16 rows make 32 operations per byte of fp16, 1/8 of what the matrix cores take for
+// each that memory gives): 656 MB of fp16 in 135.8 us, 4.84 TB/s, a large copy 4.93.  Where it is short, 7 us that do not depend on
+// its length: launch 1.4, planning 0.9 to 1.3, the first page's number 0.6, parts to the workspace 0.8 to 1.1, arrival 0.4, the
+// merge 1.6 to 2: 32 conversations of 14 heads over 2, 14 MB of int8, 8.7 us; 27 MB of Q4, 17 conversations, 14.9.
+//
+// Four wavefronts to a block; with eight those 32 conversations took 15.6 us for 9.9 (then).  A tile's memory in flight per wavefront is what its
+// registers hold, so width 64 asks for four blocks to a compute unit and 128 for two.
 
 constexpr int kRows = 16, kKeys = 32;
 constexpr int kWaves = 4;                     // wavefronts per block; they take the block's tiles in turn
@@ -673,7 +686,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kern
 //
 // What bounds it: a wavefront alone takes 1.3 us per tile at width 64, of which the matrix cores are busy 0.25 and the vector units
 // (exponentials, maxima, conversions) 0.4; the rest is the chain barrier - keys from LDS - scores - weights - values - next tile to LDS, which
-// only other wavefronts fill: matrix cores busy 22 % of the SIMD-cycles, vector units 30 %, LDS 34 % of the CU-cycles (a third of it
+// only other wavefronts fill: matrix cores busy 25 % of the SIMD-cycles, vector units 34 %, LDS 38 % of the CU-cycles (a third of it
 // bank conflicts) at 4096 rows of 32 heads over 8, width 128, window 1000 (0.55 PFLOP/s).  Tried and slower: the next tile's
 // scores under this one's weights (32 or more registers), the next tile to LDS while scores are formed, all key operands read ahead.
 
@@ -1134,6 +1147,10 @@ bool fits_a_grid(int64_t blocks, int threads) {
     return false;
 }
 
+// Three blocks per compute unit beside one per set, but no block for fewer than 16 tiles (four per wavefront).  With 1 / 2 / 3 / 4 per
+// compute unit, us: fp16, 656 MB 154 / 141 / 136.5 / 135; 16 conversations of 6676 in Q4, every head its own, 27 / 22.9 / 21.9 / 25.1; a window
+// over int8, 34 MB, 12.2 / 13.2 / 13.2 / 13.4.  With at least 8 / 16 / 32 tiles: 32 conversations in int8 10.4 / 9.2 / 11.3; 3 of 2611, every
+// head its own, 9.2 / 8.45 / 10.5.
 template <int KIND, int D>
 bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to) {
     int64_t slots = workspace ? static_cast<int64_t>(kPartialBytes / (slot_floats(D) * sizeof(float))) : 0, blocks = 0;

@@ -53,7 +53,8 @@ typedef struct mi_kv_cache {
  * q_start[b] (0: nothing of the sequence is computed).  Position p lies in page pages[b * max_pages + p / page_size], row
  * p % page_size.  Device memory: q_start [n_seqs + 1] (ascending, within 0 .. n_tokens), kv_len [n_seqs], pages
  * [n_seqs][max_pages].  n_tokens: rows that the row arrays have; rows behind q_start[n_seqs] are padding and left as they
- * are.  max_tokens: what n_b is at most, a hint by which kernels are chosen; a wrong one costs time, nothing else.
+ * are.  max_tokens: what n_b is at most, a hint; a wrong one costs time, nothing else.  The kernels are chosen
+ * by it and by max_pages * page_size, the bound of the lengths: a table much wider than that costs time for chunks of prompts.
  * Several sequences may share pages that they only read.  A position before 0, past max_pages * page_size or in a page that
  * is not in 0 .. n_pages - 1 has no place in the cache: it is not written, reads back as zeros and is not seen. */
 typedef struct mi_kv_batch {
