@@ -959,7 +959,7 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
         auto weights = [&](int c) { return __builtin_bit_cast(half8, u32x4{w[c / 2][4 * (c % 2)], w[c / 2][4 * (c % 2) + 1], w[c / 2][4 * (c % 2) + 2], w[c / 2][4 * (c % 2) + 3]}); };
         if (__builtin_expect(masked, 0)) {
             // A masked key has weight 0, but 0 x inf and 0 x NaN are NaN: where there is an infinity or a NaN in a tile that is masked
-            // for some query, the wavefront does its rows again in the end (redo), whatever comes out here.
+            // for some query, the wavefront does its rows again in the end (row_by_itself), whatever comes out here.
             uint32_t most = 0;
             #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -1176,14 +1176,15 @@ bool launch_slices(hipStream_t s, const AttentionArgs& a, void* workspace, int f
     Plan plan = make_plan(a, 32 * RW, from, 0x7fffffff, static_cast<int>(want), slots, &blocks);
     plan.least = 4;
     if (!fits_a_grid(blocks, threads)) return false;
-    auto go = [&](auto kern) {
+    auto go = [&](auto pages16) {                  // (a type of its own for each, so that each has its attribute set once)
+        const auto kern = paged_chunk_kernel<KIND, D, decltype(pages16)::value, RW, KS>;
         if (lds > 65536 && !MI_ONCE_OK(MI_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))))
             return false;
         hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(threads), lds, s, a, plan, workspace ? attention_sums(workspace) : nullptr,
                            workspace ? slice_counters(workspace) : nullptr);
         return MI_HIP_OK(hipGetLastError());
     };
-    return a.p.page.d % 16 == 0 ? go(paged_chunk_kernel<KIND, D, true, RW, KS>) : go(paged_chunk_kernel<KIND, D, false, RW, KS>);
+    return a.p.page.d % 16 == 0 ? go(std::true_type{}) : go(std::false_type{});
 }
 
 template <int KIND, int D>
