@@ -340,7 +340,9 @@ __device__ __forceinline__ bool odd_values(const Tile<KIND, D, PAGES16>& t, cons
 // merge 1.6 to 2: 32 conversations of 14 heads over 2, 14 MB of int8, 8.7 us; 27 MB of Q4, 17 conversations, 14.9.
 //
 // Four wavefronts to a block; with eight those 32 conversations took 15.6 us for 9.9 (then).  A tile's memory in flight per wavefront is what its
-// registers hold, so width 64 asks for four blocks to a compute unit and 128 for two.
+// registers hold, so width 64 asks for four blocks to a compute unit and 128 for two.  Width 64 in fp16 with pages that end inside a
+// tile asks for three: with four, 44 registers spilled (32 conversations to 4096 in pages of 100 13.8 us for 12.6, 16 to 8000 in pages of 50
+// 15.9 for 14.6); in pages of whole sixteens 3 spill, and four are as fast or faster (61 to 2500 22.7, with three 23.6).
 
 constexpr int kRows = 16, kKeys = 32;
 constexpr int kWaves = 4;                     // wavefronts per block; they take the block's tiles in turn
@@ -348,7 +350,7 @@ constexpr int slot_floats(int D) { return 16 * D + 32; }
 
 // PAGES16: pages are multiples of 16 positions long, so 16 keys lie in one page.
 template <int KIND, int D, bool PAGES16>
-__global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 4) void paged_step_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ sums,
+__global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : KIND == MI_KV_F16 && !PAGES16 ? 3 : 4) void paged_step_kernel(const AttentionArgs a, const Plan plan, float* __restrict__ sums,
                                                                  uint32_t* __restrict__ counters) {
     constexpr int kOps = D / 32, kOuts = D / 16;   // operands of a key, of the values
     constexpr int kRow = row_bytes(KIND, D), kScales = row_scales(KIND, D);
