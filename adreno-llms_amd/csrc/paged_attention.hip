@@ -1196,17 +1196,22 @@ bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int fr
     const int64_t cus = device_info().cus;
     // A set's tiles are one chain of about 1.3 us each (width 128: twice that), so where there are few sets several wavefronts take them
     // in turn.  A block of eight wavefronts is alone on its CU, of four wavefronts two are resident; sums of slices meet in LDS,
-    // of parts in memory, 33 KB per block.  Measured, us, width 64, at 128 rows / 128 in two slices / 64 in four slices:
-    //   2048 rows of 14 heads over 2 (224 sets) 28.5 / 33.7 / 33.5: blocks enough; 300 at 900, int8, 15.3 / 15.0 / 14.5; 676 of 16 over 8 in
-    //   a window of 435 (88 sets) 19.4 / 16.8 / 14.9; 14 sequences of 9 over 3 in a window of 137 21.4 / 18.6 / 16.6; 64 rows of 71, two
-    //   tiles, 8.6 / 8.0 / 8.8.
+    // of parts in memory, 33 KB per block.  Measured, us, width 64, 128 rows / 64 in four slices: 2048 rows of 14 heads over 2 (224
+    // sets) 28.5 / 33.5: blocks enough; 676 of 16 over 8 in a window of 435 (88 sets) 19.4 / 14.9; 14 sequences of 9 over 3 in a window
+    // of 137 21.4 / 16.6.
     // Width 128, 128 rows / in two slices: 17 conversations of 32 heads over 8 (208 sets) 125 / 100, 14 of 16 over 8 90 / 74; 1024 sets 109 / -.
-    if constexpr (D == 64)
-        if (sets <= cus / 2 && a.p.cap > 4 * kChunkKeys)
-            return launch_slices<KIND, D, 2, 4>(s, a, workspace, from, cus > 2 * sets ? cus - 2 * sets : 0);
-    const bool two = sets <= (D == 128 ? cus * 3 / 2 : cus / 2);
-    const int64_t want = two ? (sets < cus ? cus - sets : 0) : 2 * cus;
-    return two ? launch_slices<KIND, D, 4, 2>(s, a, workspace, from, want) : launch_slices<KIND, D, 4, 1>(s, a, workspace, from, want);
+    //
+    // Beside one block per set, as many as fill the chip, and at least half as many as it has CUs: sequences of other lengths need parts
+    // to be of one length.  None at least / half / one per CU: 32 sequences of 14 tokens to 3000 35.1 / 22.3 / 29.7; 14 of 64 tokens to 4000
+    // 41.6 / 26.9 / 32.6; 12 of 100, Q4, width 128, to 2500 60 / 41 / 53; 16 of 40 to 1500 38.1 / 35.2 / 37.4; one of 1000 tokens behind
+    // 5000 61.1 / 60.6 / 67.4; chunks and single tokens, 17 sequences, 96.8 / 97.4 / 109.
+    const int64_t half = cus / 2;
+    if constexpr (D == 64) {
+        if (sets <= half) return launch_slices<KIND, D, 2, 4>(s, a, workspace, from, std::max(cus - 2 * sets, half));
+    } else {
+        if (sets <= 3 * half) return launch_slices<KIND, D, 4, 2>(s, a, workspace, from, std::max(cus - sets, half));
+    }
+    return launch_slices<KIND, D, 4, 1>(s, a, workspace, from, 2 * cus);
 }
 
 // Which kernel.  The one for few rows reads the keys again for every 16 rows and has no start to pay for, the one for many
@@ -1216,7 +1221,7 @@ bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int fr
 //   14 heads over 2, width 64, 1 sequence: 112 sets of 16 rows at 1000 positions (14 tiles per compute unit) 8.9 / 12.4,
 //     224 (28) 11.9 / 13.6, 448 (55) 19.1 / 14.3; 28 at 16000 (55) 23.5 / 29.2, 56 (109) 35 / 25.4, 112 (219) 56 / 28.6.
 //   32 sequences: 448 sets at 500 (27) 9.9 / 11.5, 896 (55) 13.1 / 12.9, 1792 (110) 18.9 / 15.2;
-//     256 at 3000 (94) 19.8 / 20.1, 896 (328) 40 / 23.
+//     256 at 3000 (94) 19.8 / 16.9, 448 (164) 24.4 / 21.3, 896 (328) 40 / 23.
 //   32 heads over 8, width 128, 1 sequence: 256 sets at 1000 (31) 16.4 / 22.8, 512 (62) 28.8 / 23.7; 64 at 16000 (125) 47.7 / 64.2, 128 (250) 79 / 55.
 //   16 heads of their own, width 128: 512 sets at 600 (38) 15.8 / 20.8, 1024 (76) 23.8 / 21.8.
 //   300 tokens of 14 heads behind 900, int8 12.8 / 14.0.
