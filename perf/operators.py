@@ -145,15 +145,11 @@ def _decode(case, code, scale):
 
 # ---- what a program holds before the call ------------------------------------------------------------------
 
-_queue = _module = None
+_queue = None
 
 
 def _mil():
-    """The package, imported once, as a program does (a look into the import system in every call cost 3 us of it)."""
-    global _module
-    if _module is None:
-        _module = importlib.import_module("adreno-llms_amd")
-    return _module
+    return importlib.import_module("adreno-llms_amd")
 
 
 def queue():
