@@ -8,8 +8,8 @@
 // the A operand (values transposed) brings the same.  Probabilities never leave the registers.
 #include "device_math.h"
 #include "paged.h"
+#include "paged_plan.h"
 
-#include <algorithm>
 #include <type_traits>
 
 namespace mi {
@@ -105,25 +105,10 @@ __device__ __forceinline__ float element(const uint8_t* pool, const uint16_t* sc
 // one per set.  Every wavefront works that out for itself from q_start and kv_len: the loads are those that it
 // needs anyway.
 
-struct Plan {                 // from the host
-    int target;               // items per key/value head beside one per set; 0: keys are not split
-    int least;                // tiles of keys that a block is worth
-    int from, to;             // sequences of that many rows (new tokens times nrep) are the launch's
-    int nrep;
-    Divider rep;              // by nrep
-};
 struct Item {
     int b = -1, set = 0, chunk = 0, share = 0, tiles = 0;
     Span s;
 };
-
-struct Cost { int sets, tiles; };
-template <int ROWS, int KEYS>
-__device__ __forceinline__ Cost cost_of(const AttentionArgs& a, const Plan& plan, const Span& s) {
-    if (s.n <= 0 || s.n * plan.nrep < plan.from || s.n * plan.nrep > plan.to) return {0, 0};
-    const int count = tiles_of(s.pos, s.pos + s.n - 1, a.p.cap, a.window, a.sinks, KEYS).count;
-    return {(s.n * plan.nrep + ROWS - 1) / ROWS, count > 0 ? count : 1};
-}
 
 // Item `y` of the batch (of any one key/value head); b = -1: there is none.
 template <int ROWS, int KEYS>
@@ -133,21 +118,17 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
         return b < a.p.n_seqs ? span_of(a.p.q_start[b], a.p.q_start[b + 1], a.p.kv_len[b], a.p.n_tokens) : Span{};
     };
     Item it;
+    auto cost = [&](const Span& s) { return cost_of(plan, s, a.p.cap, a.window, a.sinks, ROWS, KEYS); };
     Span s = span(lane);
-    Cost c = cost_of<ROWS, KEYS>(a, plan, s);
+    Cost c = cost(s);
     it.share = 0x7fffffff;
     if (plan.target > 0) {
         float total = static_cast<float>(c.sets) * static_cast<float>(c.tiles);
         for (int b0 = 64; b0 < a.p.n_seqs; b0 += 64) {
-            const Cost more = cost_of<ROWS, KEYS>(a, plan, span(b0 + lane));
+            const Cost more = cost(span(b0 + lane));
             total += static_cast<float>(more.sets) * static_cast<float>(more.tiles);
         }
-        // (a hundred-thousandth more: the sum's rounding must not make an item too many)
-        const float all = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_to_last(total)), 63));
-        const float each = all * 1.00001f / static_cast<float>(plan.target);
-        it.share = each < 1.0e9f ? static_cast<int>(each) + 1 : 0x7fffffff;
-        if (it.share < plan.least) it.share = plan.least;
-        it.share = uniform(it.share);
+        it.share = uniform(share_of(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_to_last(total)), 63)), plan));
     }
     int before = 0;
     for (int b0 = 0;; ) {
@@ -172,7 +153,7 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
         b0 += 64;
         if (b0 >= a.p.n_seqs) return it;
         s = span(b0 + lane);
-        c = cost_of<ROWS, KEYS>(a, plan, s);
+        c = cost(s);
     }
 }
 
@@ -343,10 +324,6 @@ __device__ __forceinline__ bool odd_values(const Tile<KIND, D, PAGES16>& t, cons
 // registers hold, so width 64 asks for four blocks to a compute unit and 128 for two.  Width 64 in fp16 with pages that end inside a
 // tile asks for three: with four, 44 registers spilled (32 conversations to 4096 in pages of 100 13.8 us for 12.6, 16 to 8000 in pages of 50
 // 15.9 for 14.6); in pages of whole sixteens 3 spill, and four are as fast or faster (61 to 2500 22.7, with three 23.6).
-
-constexpr int kRows = 16, kKeys = 32;
-constexpr int kWaves = 4;                     // wavefronts per block; they take the block's tiles in turn
-constexpr int slot_floats(int D) { return 16 * D + 32; }
 
 // PAGES16: pages are multiples of 16 positions long, so 16 keys lie in one page.
 template <int KIND, int D, bool PAGES16>
@@ -692,8 +669,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : KIND == MI_KV_F16 && !P
 // bank conflicts) at 4096 rows of 32 heads over 8, width 128, window 1000 (0.55 PFLOP/s).  Tried and slower: the next tile's
 // scores under this one's weights (32 or more registers), the next tile to LDS while scores are formed, all key operands read ahead.
 
-constexpr int kChunkKeys = 64;
-constexpr int chunk_slot_floats(int D, int RW) { return 32 * RW * (D + 2); }
 constexpr int chunk_lds(int D) { return 2 * 2 * kChunkKeys * 2 * D; }          // of a slice's tiles
 constexpr int chunk_lds_all(int D, int KS) { return KS * (chunk_lds(D) + 2 * kChunkKeys); }
 constexpr int meet_floats(int D, int RW) { return RW * 64 * (D / 2 + 3); }         // of a slice's sums
@@ -1126,42 +1101,16 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
         }
 }
 
-// Blocks of a launch over sets of ROWS rows, and the plan for them: one item per set (at most one more per sequence than full
-// ones) and key/value head, and where there is a workspace for parts of sets, `want` more, as far as it reaches.
-Plan make_plan(const AttentionArgs& a, int rows_per_set, int from, int to, int want, int64_t slots, int64_t* blocks) {
-    Plan plan{};
-    plan.from = from;
-    plan.to = to;
-    plan.nrep = a.n_heads / a.p.n_kv_heads;
-    plan.rep = make_divider(plan.nrep);
-    const int64_t rows = static_cast<int64_t>(a.p.n_tokens) * plan.nrep, seqs = a.p.n_seqs < a.p.n_tokens ? a.p.n_seqs : a.p.n_tokens;
-    const int64_t sets = (rows - seqs) / rows_per_set + seqs;
-    *blocks = sets * a.p.n_kv_heads;
-    const int64_t room = slots - *blocks, target = (want < room ? want : room) / a.p.n_kv_heads;
-    plan.target = target > 0 ? static_cast<int>(target) : 0;
-    *blocks += static_cast<int64_t>(plan.target) * a.p.n_kv_heads;
-    return plan;
-}
-
-bool fits_a_grid(int64_t blocks, int threads) {
-    if (blocks <= 0xffffffffll / threads) return true;
-    MI_ERROR_FMT("mi_attention: %lld blocks are more than a launch counts", static_cast<long long>(blocks));
+bool fits_a_grid(const PagedLaunch& l) {
+    if (l.blocks <= 0xffffffffll / l.threads) return true;
+    MI_ERROR_FMT("mi_attention: %lld blocks are more than a launch counts", static_cast<long long>(l.blocks));
     return false;
 }
 
-// Three blocks per compute unit beside one per set, but no block for fewer than 16 tiles (four per wavefront).  With 1 / 2 / 3 / 4 per
-// compute unit, us: fp16, 656 MB 154 / 141 / 136.5 / 135; 16 conversations of 6676 in Q4, every head its own, 27 / 22.9 / 21.9 / 25.1; a window
-// over int8, 34 MB, 12.2 / 13.2 / 13.2 / 13.4.  With at least 8 / 16 / 32 tiles: 32 conversations in int8 10.4 / 9.2 / 11.3; 3 of 2611, every
-// head its own, 9.2 / 8.45 / 10.5.
 template <int KIND, int D>
-bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to) {
-    int64_t slots = workspace ? static_cast<int64_t>(kPartialBytes / (slot_floats(D) * sizeof(float))) : 0, blocks = 0;
-    if (slots > kSliceCounters) slots = kSliceCounters;
-    Plan plan = make_plan(a, kRows, 0, to, 3 * device_info().cus, slots, &blocks);
-    plan.least = 16;
-    if (!fits_a_grid(blocks, 64 * kWaves)) return false;
+bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
     auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, s, a, plan, workspace ? attention_sums(workspace) : nullptr,
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(l.blocks)), dim3(l.threads), 0, s, a, l.plan, workspace ? attention_sums(workspace) : nullptr,
                            workspace ? slice_counters(workspace) : nullptr);
     };
     if (a.p.page.d % 16 == 0) go(paged_step_kernel<KIND, D, true>);
@@ -1170,84 +1119,44 @@ bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, int to)
 }
 
 template <int KIND, int D, int RW, int KS>
-bool launch_slices(hipStream_t s, const AttentionArgs& a, void* workspace, int from, int64_t want) {
-    constexpr int lds = chunk_lds_all(D, KS), threads = 64 * RW * KS;
+bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
+    constexpr int lds = chunk_lds_all(D, KS);
     static_assert(lds <= 160 * 1024 && (KS - 1) * meet_floats(D, RW) * 4 <= KS * chunk_lds(D), "tiles and sums fit");
-    int64_t slots = workspace ? static_cast<int64_t>(kPartialBytes / (chunk_slot_floats(D, RW) * sizeof(float))) : 0, blocks = 0;
-    if (slots > kSliceCounters / RW) slots = kSliceCounters / RW;
-    Plan plan = make_plan(a, 32 * RW, from, 0x7fffffff, static_cast<int>(want), slots, &blocks);
-    plan.least = 4;
-    if (!fits_a_grid(blocks, threads)) return false;
     auto go = [&](auto pages16) {                  // (a type of its own for each, so that each has its attribute set once)
         const auto kern = paged_chunk_kernel<KIND, D, decltype(pages16)::value, RW, KS>;
         if (lds > 65536 && !MI_ONCE_OK(MI_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))))
             return false;
-        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(threads), lds, s, a, plan, workspace ? attention_sums(workspace) : nullptr,
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(l.blocks)), dim3(l.threads), lds, s, a, l.plan, workspace ? attention_sums(workspace) : nullptr,
                            workspace ? slice_counters(workspace) : nullptr);
         return MI_HIP_OK(hipGetLastError());
     };
     return a.p.page.d % 16 == 0 ? go(std::true_type{}) : go(std::false_type{});
 }
 
+// One of the launches that paged_plan.h chooses: of the kernel for many rows, blocks of 64 rows in four slices of keys (width 64), of
+// 128 in two (width 128) or in one.
 template <int KIND, int D>
-bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, int from) {
-    int64_t sets = 0;
-    (void)make_plan(a, 128, from, 0x7fffffff, 0, 0, &sets);
-    const int64_t cus = device_info().cus;
-    // A set's tiles are one chain of about 1.3 us each (width 128: twice that), so where there are few sets several wavefronts take them
-    // in turn.  A block of eight wavefronts is alone on its CU, of four wavefronts two are resident; sums of slices meet in LDS,
-    // of parts in memory, 33 KB per block.  Measured, us, width 64, 128 rows / 64 in four slices: 2048 rows of 14 heads over 2 (224
-    // sets) 28.5 / 33.5: blocks enough; 676 of 16 over 8 in a window of 435 (88 sets) 19.4 / 14.9; 14 sequences of 9 over 3 in a window
-    // of 137 21.4 / 16.6.
-    // Width 128, 128 rows / in two slices: 17 conversations of 32 heads over 8 (208 sets) 125 / 100, 14 of 16 over 8 90 / 74; 1024 sets 109 / -.
-    //
-    // Beside one block per set, as many as fill the chip, and at least half as many as it has CUs: sequences of other lengths need parts
-    // to be of one length.  None at least / half / one per CU: 32 sequences of 14 tokens to 3000 35.1 / 22.3 / 29.7; 14 of 64 tokens to 4000
-    // 41.6 / 26.9 / 32.6; 12 of 100, Q4, width 128, to 2500 60 / 41 / 53; 16 of 40 to 1500 38.1 / 35.2 / 37.4; one of 1000 tokens behind
-    // 5000 61.1 / 60.6 / 67.4; chunks and single tokens, 17 sequences, 96.8 / 97.4 / 109.
-    const int64_t half = cus / 2;
-    if constexpr (D == 64) {
-        if (sets <= half) return launch_slices<KIND, D, 2, 4>(s, a, workspace, from, std::max(cus - 2 * sets, half));
-    } else {
-        if (sets <= 3 * half) return launch_slices<KIND, D, 4, 2>(s, a, workspace, from, std::max(cus - sets, half));
-    }
-    return launch_slices<KIND, D, 4, 1>(s, a, workspace, from, 2 * cus);
-}
-
-// Which kernel.  The one for few rows reads the keys again for every 16 rows and has no start to pay for, the one for many
-// rows takes a tile for 64 or 128 and first fills its LDS: about 1.3 us per tile, 4 to 6 us before the first.  So what counts is
-// the work, in tiles of 16 rows by 32 keys: up to kEachCu per compute unit the whole batch is for the kernel for few rows, and
-// above that only its sequences of up to kFew rows.  Kernel for few rows / for many, us, fp16:
-//   14 heads over 2, width 64, 1 sequence: 112 sets of 16 rows at 1000 positions (14 tiles per compute unit) 8.9 / 12.4,
-//     224 (28) 11.9 / 13.6, 448 (55) 19.1 / 14.3; 28 at 16000 (55) 23.5 / 29.2, 56 (109) 35 / 25.4, 112 (219) 56 / 28.6.
-//   32 sequences: 448 sets at 500 (27) 9.9 / 11.5, 896 (55) 13.1 / 12.9, 1792 (110) 18.9 / 15.2;
-//     256 at 3000 (94) 19.8 / 16.9, 448 (164) 24.4 / 21.3, 896 (328) 40 / 23.
-//   32 heads over 8, width 128, 1 sequence: 256 sets at 1000 (31) 16.4 / 22.8, 512 (62) 28.8 / 23.7; 64 at 16000 (125) 47.7 / 64.2, 128 (250) 79 / 55.
-//   16 heads of their own, width 128: 512 sets at 600 (38) 15.8 / 20.8, 1024 (76) 23.8 / 21.8.
-//   300 tokens of 14 heads behind 900, int8 12.8 / 14.0.
-//   Up to 32 rows, at any length: 8 sequences of 28 rows at 2000 8.6 / 13.1; 32 rows, width 128, at 2000 11.9 / 19.5.
-// The host knows the lengths' bound alone, the page table's width (or the window): a table much wider than its sequences are
-// long moves them to the kernel for many rows sooner.
-constexpr int kFew = 32, kEachCu = 48;
-template <int KIND, int D>
-bool launch(hipStream_t s, const AttentionArgs& a, void* workspace) {
-    const int64_t most = static_cast<int64_t>(a.max_tokens) * (a.n_heads / a.p.n_kv_heads);
-    int64_t sets = 0, keys = a.p.cap;
-    (void)make_plan(a, kRows, 0, 0x7fffffff, 0, 0, &sets);
-    if (a.window > 0) keys = std::min(keys, static_cast<int64_t>(a.window) + a.sinks + a.max_tokens);
-    if (most <= kFew || sets * (keys / kKeys + 1) <= static_cast<int64_t>(kEachCu) * device_info().cus)
-        return launch_step<KIND, D>(s, a, workspace, 0x7fffffff);
-    if (a.p.n_seqs == 1 || static_cast<int64_t>(a.max_tokens) * a.p.n_seqs == a.p.n_tokens) return launch_chunk<KIND, D>(s, a, workspace, 0);
-    return launch_chunk<KIND, D>(s, a, workspace, kFew + 1) && launch_step<KIND, D>(s, a, workspace, kFew);
+bool launch(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
+    constexpr int kWavesSliced = D == 64 ? 2 : 4, kSlices = D == 64 ? 4 : 2;
+    if (!fits_a_grid(l)) return false;
+    if (l.wavefronts == 0) return launch_step<KIND, D>(s, a, workspace, l);
+    return l.slices == 1 ? launch_chunk<KIND, D, 4, 1>(s, a, workspace, l) : launch_chunk<KIND, D, kWavesSliced, kSlices>(s, a, workspace, l);
 }
 
 }  // namespace
 
 bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, void* workspace) {
+    const AttentionSize size = {a.p.n_seqs, a.p.n_tokens, a.max_tokens, a.p.cap, a.n_heads, a.p.n_kv_heads, a.head_dim, a.window, a.sinks};
+    const PagedLaunches all = attention_launches(size, workspace ? Room{kPartialBytes, kSliceCounters} : Room{}, device_info().cus);
     const bool wide = a.head_dim == 128;
-    if (a.kind == MI_KV_F16) return wide ? launch<MI_KV_F16, 128>(s, a, workspace) : launch<MI_KV_F16, 64>(s, a, workspace);
-    if (a.kind == MI_KV_INT8) return wide ? launch<MI_KV_INT8, 128>(s, a, workspace) : launch<MI_KV_INT8, 64>(s, a, workspace);
-    return wide ? launch<MI_KV_Q4, 128>(s, a, workspace) : launch<MI_KV_Q4, 64>(s, a, workspace);
+    for (int i = 0; i < all.n; ++i) {
+        const PagedLaunch& l = all.of[i];
+        const bool ok = a.kind == MI_KV_F16    ? wide ? launch<MI_KV_F16, 128>(s, a, workspace, l) : launch<MI_KV_F16, 64>(s, a, workspace, l)
+                        : a.kind == MI_KV_INT8 ? wide ? launch<MI_KV_INT8, 128>(s, a, workspace, l) : launch<MI_KV_INT8, 64>(s, a, workspace, l)
+                                               : wide ? launch<MI_KV_Q4, 128>(s, a, workspace, l) : launch<MI_KV_Q4, 64>(s, a, workspace, l);
+        if (!ok) return false;
+    }
+    return true;
 }
 
 }  // namespace mi
