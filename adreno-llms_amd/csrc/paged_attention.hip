@@ -1101,12 +1101,6 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
         }
 }
 
-bool fits_a_grid(const PagedLaunch& l) {
-    if (l.blocks <= 0xffffffffll / l.threads) return true;
-    MI_ERROR_FMT("mi_attention: %lld blocks are more than a launch counts", static_cast<long long>(l.blocks));
-    return false;
-}
-
 template <int KIND, int D>
 bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
     auto go = [&](auto kern) {
@@ -1138,7 +1132,6 @@ bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, const 
 template <int KIND, int D>
 bool launch(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
     constexpr int kWavesSliced = D == 64 ? 2 : 4, kSlices = D == 64 ? 4 : 2;
-    if (!fits_a_grid(l)) return false;
     if (l.wavefronts == 0) return launch_step<KIND, D>(s, a, workspace, l);
     return l.slices == 1 ? launch_chunk<KIND, D, 4, 1>(s, a, workspace, l) : launch_chunk<KIND, D, kWavesSliced, kSlices>(s, a, workspace, l);
 }
@@ -1148,6 +1141,10 @@ bool launch(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedL
 bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, void* workspace) {
     const AttentionSize size = {a.p.n_seqs, a.p.n_tokens, a.max_tokens, a.p.cap, a.n_heads, a.p.n_kv_heads, a.head_dim, a.window, a.sinks};
     const PagedLaunches all = attention_launches(size, workspace ? Room{kPartialBytes, kSliceCounters} : Room{}, device_info().cus);
+    if (const int64_t blocks = too_many_blocks(all)) {     // (of any of the launches, before the first is enqueued)
+        MI_ERROR_FMT("mi_attention: %lld blocks are more than a launch counts", static_cast<long long>(blocks));
+        return false;
+    }
     const bool wide = a.head_dim == 128;
     for (int i = 0; i < all.n; ++i) {
         const PagedLaunch& l = all.of[i];

@@ -170,4 +170,11 @@ constexpr PagedLaunches attention_launches(const AttentionSize& a, const Room& r
     return r;
 }
 
+// The blocks of a launch that has more threads than a grid counts; 0: none has.
+constexpr int64_t too_many_blocks(const PagedLaunches& all) {
+    for (int i = 0; i < all.n; ++i)
+        if (all.of[i].blocks > 0xffffffffll / all.of[i].threads) return all.of[i].blocks;
+    return 0;
+}
+
 }  // namespace mi
