@@ -110,12 +110,18 @@ struct Item {
     Span s;
 };
 
-// Item `y` of the batch (of any one key/value head); b = -1: there is none.
+// Item `y` of the batch (of any one key/value head); b = -1: there is none.  A q_start that goes down somewhere has more rows than the
+// host counted blocks for, and a set whose parts are not all there would leave its counter up for the calls to come: then no block has
+// anything (where keys are split every block looks at all of the batch; where they are not there are no counters).
 template <int ROWS, int KEYS>
 __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan, const int y) {
     const int lane = threadIdx.x & 63;
+    bool down = false;
     auto span = [&](int b) {
-        return b < a.p.n_seqs ? span_of(a.p.q_start[b], a.p.q_start[b + 1], a.p.kv_len[b], a.p.n_tokens) : Span{};
+        if (b >= a.p.n_seqs) return Span{};
+        const int start = a.p.q_start[b], end = a.p.q_start[b + 1];
+        down |= goes_down(start, end);
+        return span_of(start, end, a.p.kv_len[b], a.p.n_tokens);
     };
     Item it;
     auto cost = [&](const Span& s) { return cost_of(plan, s, a.p.cap, a.window, a.sinks, ROWS, KEYS); };
@@ -132,6 +138,7 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
     }
     int before = 0;
     for (int b0 = 0;; ) {
+        if (__any(down)) return it;
         const int chunks = c.sets ? (c.tiles - 1) / it.share + 1 : 0, upto = scan(c.sets * chunks) + before;
         const uint64_t past = __ballot(upto > y);
         if (past) {

@@ -40,6 +40,9 @@ constexpr Span span_of(int start, int end, int len, int n_tokens) {
     s.pos = (len < 0 ? 0 : len) - s.n;             // (n >= 0: no overflow; negative where a sequence has more rows than positions)
     return s;
 }
+// Whether a sequence's rows end before they begin.  Where none does, no two sequences have a row in common, and what is computed from
+// n_tokens (blocks, room for sums) is enough for all of them.
+constexpr bool goes_down(int start, int end) { return end < start; }
 
 // Positions that a table of max_pages pages has, as far as an int counts them.
 constexpr int capacity(int max_pages, int page_size) {

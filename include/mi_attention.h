@@ -55,6 +55,7 @@ typedef struct mi_kv_cache {
  * [n_seqs][max_pages].  n_tokens: rows that the row arrays have; rows behind q_start[n_seqs] are padding and left as they
  * are.  max_tokens: what n_b is at most, a hint; a wrong one costs time, nothing else.  The kernels are chosen
  * by it and by max_pages * page_size, the bound of the lengths: a table much wider than that costs time for chunks of prompts.
+ * Where q_start goes down somewhere it is not said which rows are computed, but no other memory and no later call is touched.
  * Several sequences may share pages that they only read.  A position before 0, past max_pages * page_size or in a page that
  * is not in 0 .. n_pages - 1 has no place in the cache: it is not written, reads back as zeros and is not seen. */
 typedef struct mi_kv_batch {

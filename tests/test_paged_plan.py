@@ -26,6 +26,8 @@ extern "C" int launches(const int* v, int room, int cus, int* out) {
     }
     return r.n;
 }
+extern "C" int down(int start, int end) { return goes_down(start, end); }
+extern "C" int span_n(int start, int end, int rows) { return span_of(start, end, 0, rows).n; }
 // items of a launch over the sequences (rows n, positions len each), and the greatest number of parts of a set
 extern "C" void items(const int* v, const int* l, const int* n, const int* len, long long* out) {
     Plan plan;
@@ -80,7 +82,7 @@ def rule(tmp_path_factory):
         return list(out)
 
     rule = lambda: None                                                            # noqa: E731
-    rule.launches, rule.items = launches, items
+    rule.launches, rule.items, rule.down, rule.span_n = launches, items, lib.down, lib.span_n
     return rule
 
 
@@ -133,3 +135,26 @@ def test_a_launch_counts_its_own_sequences(rule):
     # and a batch of which nothing can be long enough for the kernel for many rows, whatever the hint says
     one, = rule.launches(**dict(_size([1] * 3, [100000] * 3), max_tokens=4096, cap=2 ** 24))
     assert one.wavefronts == 0 and one.last >= 12
+
+
+def test_rows_that_no_two_sequences_share(rule):
+    """Wherever q_start does not go down, whatever else it holds, the sequences' rows are no more than the batch's; one that goes down
+    has more, so it has to be told apart."""
+    rng = random.Random(4)
+    big, ups, more = 2 ** 31 - 1, 0, 0
+    for _ in range(20000):
+        rows = rng.choice([1, 7, 100])
+        start = [rng.choice([-big, -1, 0, 0, 3, 5, 7, 50, 100, 101, big]) for _ in range(rng.randint(2, 6))]
+        if rng.random() < 0.5:
+            start.sort()
+        down = any(rule.down(s, e) for s, e in zip(start, start[1:]))
+        all_rows = sum(rule.span_n(s, e, rows) for s, e in zip(start, start[1:]))
+        ups += not down
+        more += all_rows > rows
+        assert down or all_rows <= rows
+    assert ups > 5000 and more > 500
+    # the blocks of such a call would not be all there: 6 sequences of the same 5 rows, counted as 5 rows
+    size = dict(_size([5] * 6, [3000] * 6, heads=14, kv=2, D=64), n_tokens=5, max_tokens=1)
+    one, = rule.launches(**size)
+    n, sets, parts = rule.items(one, [5] * 6, [3000] * 6, **dict(size, n_tokens=30))
+    assert parts > 1 and sets > one.each - one.target and any(rule.down(s, e) for s, e in zip([0, 5, 0], [5, 0, 5]))
