@@ -30,6 +30,19 @@ constexpr float kStart = -1.0e30f;               // the running maximum of a que
 // above it: so the greatest weight is between 2^7 and 2^15, fp16 holds weights down to 2^-21 of it at full precision, and the sums
 // are rescaled only where the maximum has risen by more than kSlack.
 constexpr float kHead = 7.0f, kSlack = 8.0f;
+// Up to there (2^23, where fp32 counts in halves) a score times scale goes into its weight's exponent unrounded, by fma.  Beyond, what an
+// unrounded product is apart from a rounded base may be more than fp16's whole range, so each product is rounded first: equal
+// scores then have equal weights, of at most 2^kMost (a product just over base + kSlack + kHead may round to it; fp16 ends below 2^16).
+constexpr float kFar = 8388608.0f, kMost = 15.9375f;
+__device__ __forceinline__ float far_exponent(float score, float scale_log2, float base) {
+    const float x = fabsf(base) < kFar ? fmaf(score, scale_log2, -base) : score * scale_log2 - base;
+    return x > kMost ? kMost : x;                    // (a NaN stays one)
+}
+// The base for a greatest score `most`, from the product as far_exponent has it.
+__device__ __forceinline__ float base_of(float most, float scale_log2) {
+    const float rounded = most * scale_log2 - kHead;
+    return fabsf(rounded) < kFar ? fmaf(most, scale_log2, -kHead) : rounded;
+}
 
 // The greater of a lane's value and those of the lanes 16, 32 and 48 away.
 __device__ __forceinline__ float max_of_groups(float a) {
@@ -468,6 +481,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : KIND == MI_KV_F16 && !P
     #pragma unroll
     for (int e = 0; e < 8; ++e) ones[e] = static_cast<_Float16>(1.0f);
     const float scale_log2 = a.scale * 1.44269504088896341f;
+    bool far = false;                              // some query's base is beyond kFar
 
     // Tile v, whose rows are `r`; `more`: the keys and values of tile v + kWaves, at `next`, are asked for as soon as the registers of
     // tile v's are free, so that they are on their way meanwhile without registers of their own.
@@ -497,18 +511,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : KIND == MI_KV_F16 && !P
             }
         }
         float top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max3(s[1][2], s[1][3], s[1][3]));
-        top = fmaf(top, scale_log2, -kHead);
-        if (__builtin_expect(__any(top > base + kSlack), 0)) {
-            top = fmaxf(base, max_of_groups(top));
+        if (__builtin_expect(__any(top * scale_log2 - kHead > base + kSlack), 0)) {
+            top = fmaxf(base, max_of_groups(base_of(top, scale_log2)));
             const float alpha = __builtin_amdgcn_exp2f(base - top);
             l *= alpha;
             #pragma unroll
             for (int m = 0; m < kOuts; ++m) acc[m] *= alpha;
             base = top;
+            far = __any(fabsf(base) >= kFar && base > kStart);
+        }
+        float by = scale_log2, from = base;
+        if (__builtin_expect(far, 0)) {
+            asm volatile("");
+            #pragma unroll
+            for (int e = 0; e < 8; ++e) s[e / 4][e % 4] = far_exponent(s[e / 4][e % 4], scale_log2, base);
+            by = 1.0f;
+            from = 0.0f;
         }
         float w[8];
         #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], scale_log2, -base));
+        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[e / 4][e % 4], by, -from));
         pack_scales(t, i);
         const half8 pb = __builtin_bit_cast(half8, u32x4{pack2(w[0], w[1]), pack2(w[2], w[3]), pack2(w[4], w[5]), pack2(w[6], w[7])});
         l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pb, l, 0, 0, 0);
@@ -705,7 +727,7 @@ __device__ __forceinline__ void row_by_itself(const AttentionArgs& a, const int*
                 float dot = 0.0f;
                 #pragma unroll 1
                 for (int e = 0; e < D; ++e) dot = fmaf(h_f(q[e]), element<KIND, D>(a.p.k, a.p.k_scale, at, e), dot);
-                score = dot * a.scale * 1.44269504088896341f;
+                score = dot * (a.scale * 1.44269504088896341f);
             }
         }
         const float now = fmaxf(base, wave_max(score) - kHead), was = __builtin_amdgcn_exp2f(base - now);
@@ -867,7 +889,7 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
     // lane addresses within a tile: of a key operand, piece 2 j + h of row i; of a value operand, 4 rows of 16 elements for 16 lanes
     const int vr = 4 * h + (lane & 15) / 4, vc = (lane >> 4 & 1) * 2 + (lane & 3) / 2, vo = (lane & 1) * 8;
 
-    bool odd = false;                              // see below
+    bool odd = false, far = false;                 // see below; some query's base is beyond kFar
     auto multiply = [&](int v, int buf) {
         const int j0 = tile_at(tiles, v) * kChunkKeys;
         const uint8_t* const kt = own_lds + buf * (chunk_lds(D) / 2);
@@ -904,9 +926,8 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
             #pragma unroll
             for (int z = 0; z < 4; ++z) tops[z] = max3(tops[z], s[z / 2][8 * (z % 2) + r], s[z / 2][8 * (z % 2) + r + 1]);
         float top = max3(max3(tops[0], s[0][7], tops[1]), max3(s[0][15], tops[2], s[1][7]), max3(tops[3], s[1][15], s[1][15]));
-        top = fmaf(top, scale_log2, -kHead);
-        if (__builtin_expect(__any(top > base + kSlack), 0)) {
-            unsigned u = __float_as_uint(top);
+        if (__builtin_expect(__any(top * scale_log2 - kHead > base + kSlack), 0)) {
+            unsigned u = __float_as_uint(base_of(top, scale_log2));
             const auto both_halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);
             top = max3(base, __uint_as_float(both_halves[0]), __uint_as_float(both_halves[1]));
             const float alpha = __builtin_amdgcn_exp2f(base - top);
@@ -914,6 +935,17 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
             #pragma unroll
             for (int m = 0; m < kOuts; ++m) acc[m] *= alpha;
             base = top;
+            far = __any(fabsf(base) >= kFar && base > kStart);
+        }
+        float by = scale_log2, from = base;
+        if (__builtin_expect(far, 0)) {
+            asm volatile("");
+            #pragma unroll
+            for (int t = 0; t < 2; ++t)
+                #pragma unroll
+                for (int r = 0; r < 16; ++r) s[t][r] = far_exponent(s[t][r], scale_log2, base);
+            by = 1.0f;
+            from = 0.0f;
         }
         uint32_t w[2][8];                          // weights, two to a word
         float sums[4] = {sum, 0.0f, 0.0f, 0.0f};
@@ -921,7 +953,7 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
         for (int t = 0; t < 2; ++t)
             #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                w[t][r / 2] = pack2(__builtin_amdgcn_exp2f(fmaf(s[t][r], scale_log2, -base)), __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], scale_log2, -base)));
+                w[t][r / 2] = pack2(__builtin_amdgcn_exp2f(fmaf(s[t][r], by, -from)), __builtin_amdgcn_exp2f(fmaf(s[t][r + 1], by, -from)));
                 float& part = sums[2 * t + r / 2 % 2];
                 part = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, w[t][r / 2]), half2v{static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)}, part, false);
             }
