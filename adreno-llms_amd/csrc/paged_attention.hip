@@ -665,11 +665,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : KIND == MI_KV_F16 && !P
         }
     }
     if (!live) return;
-    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    const float inv = __fdiv_rn(1.0f, sum);        // (not used where the sum is 0)
     uint16_t* const dst = a.out + (it.s.first + token) * a.ld_out + head * D + element;
     uint32_t h[kMine / 2];
     #pragma unroll
-    for (int m = 0; m < kMine; m += 2) h[m / 2] = pack2(o[m] * inv, o[m + 1] * inv);
+    for (int m = 0; m < kMine; m += 2) h[m / 2] = sum == 0.0f ? 0u : pack2(o[m] * inv, o[m + 1] * inv);      // (o may be NaN)
     if (reinterpret_cast<uintptr_t>(dst) % (2 * kMine) == 0) {
         if constexpr (kMine == 8) *reinterpret_cast<u32x4*>(dst) = u32x4{h[0], h[1], h[2], h[3]};
         else if constexpr (kMine == 4) *reinterpret_cast<u32x2*>(dst) = u32x2{h[0], h[1]};
@@ -1122,14 +1122,15 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
         }
     }
     if (!live) return;
-    const float inv = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+    const float inv = __fdiv_rn(1.0f, sum);        // (not used where the sum is 0)
     uint16_t* const dst = a.out + (it.s.first + token) * a.ld_out + head * D + 4 * h;
     const bool wide = reinterpret_cast<uintptr_t>(dst) % 8 == 0;
     #pragma unroll
     for (int m = 0; m < kOuts; ++m)
         #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const u32x2 x = {pack2(acc[m][4 * e] * inv, acc[m][4 * e + 1] * inv), pack2(acc[m][4 * e + 2] * inv, acc[m][4 * e + 3] * inv)};
+            u32x2 x = {pack2(acc[m][4 * e] * inv, acc[m][4 * e + 1] * inv), pack2(acc[m][4 * e + 2] * inv, acc[m][4 * e + 3] * inv)};
+            if (sum == 0.0f) x = u32x2{0, 0};      // (acc may be NaN)
             uint16_t* const to = dst + 32 * m + 8 * e;
             if (wide) {
                 *reinterpret_cast<u32x2*>(to) = x;

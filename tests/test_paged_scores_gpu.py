@@ -77,3 +77,14 @@ def test_one_key_above_all_others_far_from_0(monkeypatch, queue, kind, at, form)
     if kind == mil.KV_INT8:                              # (6 of 7 is 108.9 codes of 127: the rows are still alike)
         assert (c.pool["k"][c.table[0, 0]][:, 1] == 109).any()
     _check(c, c.upload().attend(queue, scale=0.123), want, mean)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("odd", [1.0, np.inf, np.nan])
+def test_scores_of_minus_infinity_alone_give_zeros(monkeypatch, queue, odd, form):
+    """Whatever the values are."""
+    c = _cache(monkeypatch, mil.KV_F16, 64, form, 1.0, 0.0)
+    c.k[0][:, :, 5] = -np.inf
+    c.v[0][::3, :, 7] = odd
+    c.fill()
+    assert (c.upload().attend(queue).view(np.uint16) & 0x7fff == 0).all()
