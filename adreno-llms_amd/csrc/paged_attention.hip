@@ -1015,7 +1015,7 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
         if (v < last) {
             const int j0 = tile_at(tiles, v) * kChunkKeys;
             const int w_first = a.window > 0 && p_lo >= a.window ? p_lo - a.window + 1 : 0;    // of the window of the wavefront's first query
-            if (busy && j0 <= p_hi && (j0 + kChunkKeys > w_first || j0 < sinks)) multiply(v, buf);
+            if (busy && j0 <= p_hi && (j0 + (kChunkKeys - 1) >= w_first || j0 < sinks)) multiply(v, buf);
         }
     }
     if constexpr (KS > 1) {
