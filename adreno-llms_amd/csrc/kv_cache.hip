@@ -197,6 +197,10 @@ unsigned blocks_for(const char* who, const PagedArgs& a) {
 
 bool bad_rows(const char* who, const void* k, int ld_k, const void* v, int ld_v, const PagedArgs& a, int D) {
     const int64_t width = static_cast<int64_t>(a.n_kv_heads) * D;
+    if (width > 0x7fffffff - 64 * kPiece) {            // (the kernels count elements of a row in ints, a wavefront's past the last)
+        MI_ERROR_FMT("%s: rows of %lld elements are more than a launch counts", who, static_cast<long long>(width));
+        return true;
+    }
     if (k && v && ld_k >= width && ld_v >= width && reinterpret_cast<uintptr_t>(k) % 2 == 0 && reinterpret_cast<uintptr_t>(v) % 2 == 0)
         return false;
     MI_ERROR_FMT("%s: bad rows (k=%p ld_k=%d v=%p ld_v=%d, %lld elements each)", who, k, ld_k, v, ld_v, static_cast<long long>(width));
