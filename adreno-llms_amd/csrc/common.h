@@ -1,5 +1,7 @@
 // Shared declarations of the host layer and the kernel launchers.
 #pragma once
+#include "stream_room.h"
+
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>
@@ -126,8 +128,8 @@ WeightEntry weight_entry(const void* W);
 uint64_t registry_epoch();
 // The workspace of a stream that mi_stream_create made (null: another stream, or no memory was left for one)
 void* own_stream_workspace(hipStream_t s);
-// The same, of the null stream as well
-void* stream_workspace(hipStream_t s);
+// All that such a stream has, and the null stream
+StreamRoom stream_room(hipStream_t s);
 // While it lives, launches that this thread enqueues on `recording` (a stream of the library's own, under capture) use the
 // workspace and the modes of `s`, the stream that the recording will be replayed on.  One at a time in a thread.
 class StandsFor {
@@ -182,17 +184,6 @@ GemmRoute gemm_route(hipStream_t s, const GemvCall& c, size_t workspace_bytes);
 // n calls of one M and weight kind and of GemmRoute::kShares (up to 64 rows, or in tiles of rows), of any x, K and N, none of which reads or writes what
 // another one writes: in one launch where they fit it, each result what launch_gemm gives.
 bool launch_gemm_many(hipStream_t s, const GemvCall* calls, int n, void* workspace, size_t workspace_bytes);
-// A stream's workspace holds kWorkspaceBytes for whatever a launch puts there and, behind them, kSliceCounters
-// counters that are 0 between launches (slices of K that meet inside a launch).
-constexpr size_t kWorkspaceBytes = 16u << 20;
-constexpr int kSliceCounters = 16384;
-inline uint32_t* slice_counters(void* workspace) {
-    return reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kWorkspaceBytes);
-}
-// Behind the counters: room for the sums of attention's rows whose keys several blocks share (paged_attention.hip).
-constexpr size_t kPartialBytes = 32u << 20;
-inline float* attention_sums(void* workspace) { return reinterpret_cast<float*>(slice_counters(workspace) + kSliceCounters); }
-constexpr size_t kAllWorkspaceBytes = kWorkspaceBytes + kSliceCounters * sizeof(uint32_t) + kPartialBytes;
 // runtime.hip: the same for a registered W where mi_linear would run the GEMM
 int linear_glu(hipStream_t s, int M, int N, int K, const void* x, const void* W, void* out);
 // gemm.hip, runtime.hip: the sums of the K slices of a GEMM that mi_linear would cut into slices, left in the stream's

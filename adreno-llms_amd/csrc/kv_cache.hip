@@ -333,5 +333,5 @@ extern "C" int mi_attention(void* stream, const mi_attention_call* call) {
     a.sinks = c.sinks;
     a.scale = c.scale;
     const auto s = static_cast<hipStream_t>(stream);
-    return launch_paged_attention(s, a, stream_workspace(s)) ? 1 : 0;
+    return launch_paged_attention(s, a, stream_room(s)) ? 1 : 0;
 }

@@ -37,6 +37,6 @@ struct AttentionArgs {
     int window, sinks;
     float scale;
 };
-bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, void* workspace);
+bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, const StreamRoom& room);
 
 }  // namespace mi

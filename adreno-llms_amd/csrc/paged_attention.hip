@@ -1141,11 +1141,15 @@ __global__ __launch_bounds__(64 * RW * KS, 2) void paged_chunk_kernel(const Atte
         }
 }
 
+struct PartRoom {             // of the stream: where parts of a sequence's keys meet (null: nowhere)
+    float* sums = nullptr;
+    uint32_t* counters = nullptr;
+};
+
 template <int KIND, int D>
-bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
+bool launch_step(hipStream_t s, const AttentionArgs& a, const PartRoom& room, const PagedLaunch& l) {
     auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(l.blocks)), dim3(l.threads), 0, s, a, l.plan, workspace ? attention_sums(workspace) : nullptr,
-                           workspace ? slice_counters(workspace) : nullptr);
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(l.blocks)), dim3(l.threads), 0, s, a, l.plan, room.sums, room.counters);
     };
     if (a.p.page.d % 16 == 0) go(paged_step_kernel<KIND, D, true>);
     else go(paged_step_kernel<KIND, D, false>);
@@ -1153,15 +1157,14 @@ bool launch_step(hipStream_t s, const AttentionArgs& a, void* workspace, const P
 }
 
 template <int KIND, int D, int RW, int KS>
-bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
+bool launch_chunk(hipStream_t s, const AttentionArgs& a, const PartRoom& room, const PagedLaunch& l) {
     constexpr int lds = chunk_lds_all(D, KS);
     static_assert(lds <= 160 * 1024 && (KS - 1) * meet_floats(D, RW) * 4 <= KS * chunk_lds(D), "tiles and sums fit");
     auto go = [&](auto pages16) {                  // (a type of its own for each, so that each has its attribute set once)
         const auto kern = paged_chunk_kernel<KIND, D, decltype(pages16)::value, RW, KS>;
         if (lds > 65536 && !MI_ONCE_OK(MI_HIP_OK(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds))))
             return false;
-        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(l.blocks)), dim3(l.threads), lds, s, a, l.plan, workspace ? attention_sums(workspace) : nullptr,
-                           workspace ? slice_counters(workspace) : nullptr);
+        hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(l.blocks)), dim3(l.threads), lds, s, a, l.plan, room.sums, room.counters);
         return MI_HIP_OK(hipGetLastError());
     };
     return a.p.page.d % 16 == 0 ? go(std::true_type{}) : go(std::false_type{});
@@ -1170,17 +1173,19 @@ bool launch_chunk(hipStream_t s, const AttentionArgs& a, void* workspace, const 
 // One of the launches that paged_plan.h chooses: of the kernel for many rows, blocks of 64 rows in four slices of keys (width 64), of
 // 128 in two (width 128) or in one.
 template <int KIND, int D>
-bool launch(hipStream_t s, const AttentionArgs& a, void* workspace, const PagedLaunch& l) {
+bool launch(hipStream_t s, const AttentionArgs& a, const PartRoom& room, const PagedLaunch& l) {
     constexpr int kWavesSliced = D == 64 ? 2 : 4, kSlices = D == 64 ? 4 : 2;
-    if (l.wavefronts == 0) return launch_step<KIND, D>(s, a, workspace, l);
-    return l.slices == 1 ? launch_chunk<KIND, D, 4, 1>(s, a, workspace, l) : launch_chunk<KIND, D, kWavesSliced, kSlices>(s, a, workspace, l);
+    if (l.wavefronts == 0) return launch_step<KIND, D>(s, a, room, l);
+    return l.slices == 1 ? launch_chunk<KIND, D, 4, 1>(s, a, room, l) : launch_chunk<KIND, D, kWavesSliced, kSlices>(s, a, room, l);
 }
 
 }  // namespace
 
-bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, void* workspace) {
+bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, const StreamRoom& own) {
+    PartRoom room;
+    if (own.workspace && own.sums) room = {static_cast<float*>(own.sums), slice_counters(own.workspace)};
     const AttentionSize size = {a.p.n_seqs, a.p.n_tokens, a.max_tokens, a.p.cap, a.n_heads, a.p.n_kv_heads, a.head_dim, a.window, a.sinks};
-    const PagedLaunches all = attention_launches(size, workspace ? Room{kPartialBytes, kSliceCounters} : Room{}, device_info().cus);
+    const PagedLaunches all = attention_launches(size, room.sums ? Room{kPartialBytes, kSliceCounters} : Room{}, device_info().cus);
     if (const int64_t blocks = too_many_blocks(all)) {     // (of any of the launches, before the first is enqueued)
         MI_ERROR_FMT("mi_attention: %lld blocks are more than a launch counts", static_cast<long long>(blocks));
         return false;
@@ -1188,9 +1193,9 @@ bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, void* workspa
     const bool wide = a.head_dim == 128;
     for (int i = 0; i < all.n; ++i) {
         const PagedLaunch& l = all.of[i];
-        const bool ok = a.kind == MI_KV_F16    ? wide ? launch<MI_KV_F16, 128>(s, a, workspace, l) : launch<MI_KV_F16, 64>(s, a, workspace, l)
-                        : a.kind == MI_KV_INT8 ? wide ? launch<MI_KV_INT8, 128>(s, a, workspace, l) : launch<MI_KV_INT8, 64>(s, a, workspace, l)
-                                               : wide ? launch<MI_KV_Q4, 128>(s, a, workspace, l) : launch<MI_KV_Q4, 64>(s, a, workspace, l);
+        const bool ok = a.kind == MI_KV_F16    ? wide ? launch<MI_KV_F16, 128>(s, a, room, l) : launch<MI_KV_F16, 64>(s, a, room, l)
+                        : a.kind == MI_KV_INT8 ? wide ? launch<MI_KV_INT8, 128>(s, a, room, l) : launch<MI_KV_INT8, 64>(s, a, room, l)
+                                               : wide ? launch<MI_KV_Q4, 128>(s, a, room, l) : launch<MI_KV_Q4, 64>(s, a, room, l);
         if (!ok) return false;
     }
     return true;

@@ -42,11 +42,11 @@ std::unordered_map<const void*, Entry> g_registry;
 std::mutex g_registry_mu;
 std::atomic<uint64_t> g_registry_epoch{0};
 
-// One GEMM workspace per stream made by mi_stream_create, and one for the null stream made by
+// One workspace per stream made by mi_stream_create, and one for the null stream made by
 // mi_init: allocated there, never inside a compute call.  Work on one stream is ordered, so the
-// calls of a stream can share its workspace; a stream from elsewhere has none and its GEMMs
-// simply do not slice K.
-std::unordered_map<hipStream_t, void*> g_workspace;
+// calls of a stream can share its workspace; a stream from elsewhere has none: its GEMMs
+// simply do not slice K, and its attention does not split keys.
+std::unordered_map<hipStream_t, StreamRoom> g_workspace;
 struct StreamModes { int gemv = -1, gemm = -1; };      // -1: the process default
 std::unordered_map<hipStream_t, StreamModes> g_stream_modes;
 
@@ -58,11 +58,12 @@ void* g_static_scratch[kMaxDevices] = {};     // device address of `scratch` per
 thread_local hipStream_t t_recording = nullptr, t_stands_for = nullptr;      // StandsFor
 hipStream_t stood_for(hipStream_t s) { return s && s == t_recording ? t_stands_for : s; }
 
-void* workspace_of(hipStream_t s) {
+StreamRoom room_of(hipStream_t s) {
     std::lock_guard<std::mutex> lk(g_registry_mu);
     auto it = g_workspace.find(stood_for(s));
-    return it == g_workspace.end() ? nullptr : it->second;
+    return it == g_workspace.end() ? StreamRoom{} : it->second;
 }
+void* workspace_of(hipStream_t s) { return room_of(s).workspace; }
 
 // On a stream that goes again, and waited for: cleared on the streams themselves, the null stream among them, by a memset or a
 // fill kernel, or by a copy on the null stream, they made every later launch of the program slower (the Q4 lm_head with its
@@ -77,14 +78,22 @@ bool clear_counters(void* workspace) {
 }
 
 void add_workspace(hipStream_t s) {
-    void* p = nullptr;
-    if (hipMalloc(&p, kAllWorkspaceBytes) != hipSuccess || !clear_counters(p)) {
-        (void)hipGetLastError();      // no workspace: that stream's GEMMs run unsliced
-        (void)hipFree(p);
-        return;
-    }
+    const StreamRoom r = make_stream_room(
+        [](size_t bytes) {
+            void* p = nullptr;
+            if (hipMalloc(&p, bytes) == hipSuccess) return p;
+            (void)hipGetLastError();
+            return static_cast<void*>(nullptr);
+        },
+        [](void* workspace) {
+            const bool ok = clear_counters(workspace);
+            if (!ok) (void)hipGetLastError();
+            return ok;
+        },
+        [](void* p) { (void)hipFree(p); });
+    if (!r.workspace) return;
     std::lock_guard<std::mutex> lk(g_registry_mu);
-    g_workspace[s] = p;
+    g_workspace[s] = r;
 }
 
 bool lookup(const void* W, Entry* out) {
@@ -137,7 +146,7 @@ WeightEntry weight_entry(const void* W) {
 uint64_t registry_epoch() { return g_registry_epoch.load(); }
 
 void* own_stream_workspace(hipStream_t s) { return s ? workspace_of(s) : nullptr; }
-void* stream_workspace(hipStream_t s) { return workspace_of(s); }
+StreamRoom stream_room(hipStream_t s) { return room_of(s); }
 
 StandsFor::StandsFor(hipStream_t recording, hipStream_t s) {
     t_recording = recording;
@@ -297,17 +306,18 @@ int mi_stream_destroy(void* s) {
     // (whoever finds the stream gone from the tables may take its work to be over)
     if (hipStreamSynchronize(as_stream(s)) != hipSuccess) (void)hipGetLastError();
     const int ok = MI_HIP_OK(hipStreamDestroy(as_stream(s))) ? 1 : 0;
-    void* ws = nullptr;
+    StreamRoom room;
     {
         std::lock_guard<std::mutex> lk(g_registry_mu);
         auto it = g_workspace.find(as_stream(s));
         if (it != g_workspace.end()) {
-            ws = it->second;
+            room = it->second;
             g_workspace.erase(it);
         }
         g_stream_modes.erase(as_stream(s));
     }
-    if (ws) (void)hipFree(ws);
+    if (room.workspace) (void)hipFree(room.workspace);
+    if (room.sums) (void)hipFree(room.sums);
     return ok;
 }
 int mi_stream_sync(void* s) { return MI_HIP_OK(hipStreamSynchronize(as_stream(s))) ? 1 : 0; }
