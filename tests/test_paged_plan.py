@@ -158,3 +158,22 @@ def test_rows_that_no_two_sequences_share(rule):
     one, = rule.launches(**size)
     n, sets, parts = rule.items(one, [5] * 6, [3000] * 6, **dict(size, n_tokens=30))
     assert parts > 1 and sets > one.each - one.target and any(rule.down(s, e) for s, e in zip([0, 5, 0], [5, 0, 5]))
+
+
+def test_cases_come_to_the_kernels_that_they_are_for(rule):
+    """On 256 compute units, those of the device that they are written for."""
+    from helpers import mil                                                        # noqa: F401
+    from test_paged_kernels_gpu import FEW, MANY, WIDE
+
+    def of(case, page, columns=0, **more):
+        pages = max(-(-max(case["lengths"]) // page), columns // page)
+        size = _size(case["new"], case["lengths"], case["heads"], case["kv_heads"], case["D"], pad=case.get("pad", 0), cap=pages * page, **more)
+        return rule.launches(**size)
+
+    for (D, slices), (case, columns) in MANY.items():
+        for page in (16, 100, 48, 5):
+            many, few = of(case, page, columns)
+            assert (many.wavefronts, many.slices, few.wavefronts) == (2 if slices == 4 else 4, slices, 0), (D, slices, page)
+    for case in FEW.values():
+        assert [x.wavefronts for x in of(case, 16)] == [0]
+    assert WIDE == 2 ** 20
