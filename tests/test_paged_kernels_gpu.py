@@ -1,5 +1,5 @@
 """Every kernel of mi_attention by itself (which one a call comes to is paged_plan.h's; test_paged_plan.py looks that these cases come
-to the ones they are for)."""
+to the ones they are for), and what masked places hold under a window in the one for many rows."""
 import numpy as np
 import pytest
 
@@ -18,6 +18,11 @@ MANY = {
     (128, 1): (dict(heads=16, kv_heads=8, D=128, lengths=[500, 90, 400], new=[100, 90, 1], pad=3200), 0),
 }
 FEW = {D: dict(heads=8, kv_heads=4, D=D, lengths=[700, 33, 400], new=[1, 9, 1]) for D in (64, 128)}
+# Under a window: two sequences of which many rows share tiles; (slices, rows of padding, window, sinks)
+UNDER_WINDOW = [(1, 3500, 16, 4), (1, 3500, 3, 0), (1, 3500, 64, 64), (1, 3500, 1, 1), (1, 3500, 100, 37), (4, 1450, 200, 5), (4, 1450, 200, 0),
+                (4, 1450, 215, 130)]
+WINDOW_CACHE = dict(heads=8, kv_heads=4, D=64, page=16, lengths=[500, 300], new=[250, 200])
+
 
 @pytest.fixture(scope="module")
 def queue():
@@ -41,3 +46,35 @@ def test_many_rows(monkeypatch, queue, kind, D, slices, page):
 def test_few_rows(queue, kind, D, page):
     c = Cache(kind, page=page, seed=62, **FEW[D]).upload()
     c.check(c.attend(queue))
+
+
+@pytest.mark.parametrize("slices,pad,window,sinks", UNDER_WINDOW)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("kind", KINDS)
+def test_what_a_window_leaves_behind_does_not_matter(queue, kind, bad, slices, pad, window, sinks):
+    """Infinities and NaN among the values: at the causal edge and behind the window (key/value heads 0 and 1), right behind the sinks (2),
+    and in a sink, where there is one (3: every row sees it).  Rows that see none are as ever, the others have it."""
+    c = Cache(kind, seed=63, pad=pad, **WINDOW_CACHE)
+    places = {0: [494], 1: [255, 490], 2: [sinks], 3: [0]}
+    for head, at in places.items():
+        c.v[0][at, head, 9] = bad
+    c.k[0][260, 0, 5] = np.nan                              # and a key
+    places[0] = [494, 260]
+    c.fill()
+    got = c.upload().attend(queue, window=window, sinks=sinks)
+    want, tol = c.expect(window, sinks)
+    p = np.arange(250, 500)
+    for head, at in places.items():
+        sees = np.zeros((250, len(at)), bool)
+        for i, j in enumerate(at):
+            sees[:, i] = (j <= p) & ((j > p - window) | (j < sinks))
+        clean, own = ~sees.any(1), slice(2 * head, 2 * head + 2)
+        off = np.abs(got[:250, own].astype(np.float64) - want[:250, own]) <= tol[:250, own]
+        assert off[clean].all(), (head, np.nonzero(~off & clean[:, None, None])[0][:5])
+        seen = sees[:, [j != 260 for j in at]].any(1)
+        assert not np.isfinite(got[:250, own, 9][seen]).any()
+        if head == 0:
+            assert np.isnan(got[:250, own][sees[:, 1]]).all()
+        assert head == 3 or clean.sum() >= 15, "the test has to have rows to look at"
+    rest = slice(250, 450)
+    assert (np.abs(got[rest].astype(np.float64) - want[rest]) <= tol[rest]).all()

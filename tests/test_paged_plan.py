@@ -163,7 +163,7 @@ def test_rows_that_no_two_sequences_share(rule):
 def test_cases_come_to_the_kernels_that_they_are_for(rule):
     """On 256 compute units, those of the device that they are written for."""
     from helpers import mil                                                        # noqa: F401
-    from test_paged_kernels_gpu import FEW, MANY, WIDE
+    from test_paged_kernels_gpu import FEW, MANY, UNDER_WINDOW, WIDE, WINDOW_CACHE
 
     def of(case, page, columns=0, **more):
         pages = max(-(-max(case["lengths"]) // page), columns // page)
@@ -176,4 +176,7 @@ def test_cases_come_to_the_kernels_that_they_are_for(rule):
             assert (many.wavefronts, many.slices, few.wavefronts) == (2 if slices == 4 else 4, slices, 0), (D, slices, page)
     for case in FEW.values():
         assert [x.wavefronts for x in of(case, 16)] == [0]
+    for slices, pad, window, sinks in UNDER_WINDOW:
+        many = of(dict(WINDOW_CACHE, pad=pad), 16, window=window, sinks=sinks)[0]
+        assert many.wavefronts and many.slices == slices, (pad, window, sinks)
     assert WIDE == 2 ** 20
