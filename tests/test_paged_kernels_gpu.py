@@ -78,3 +78,21 @@ def test_what_a_window_leaves_behind_does_not_matter(queue, kind, bad, slices, p
         assert head == 3 or clean.sum() >= 15, "the test has to have rows to look at"
     rest = slice(250, 450)
     assert (np.abs(got[rest].astype(np.float64) - want[rest]) <= tol[rest]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 70])
+def test_small_weights_count(queue, kind, n):
+    """9000 positions at 2^-22 of the greatest weight, 0.2 % of its sum, with values a hundred times as large: a sixth of the output,
+    many times what it may be off by."""
+    c = Cache(kind, 14, 2, 64, 32, [9000], [n], seed=64)
+    c.qkv[:, :14 * 64] = 1.0                                # q k: scores 15.2 and 0
+    c.k[0][:] = 0
+    c.k[0][17] = 1.9
+    c.v[0][:] = np.abs(c.v[0]) * 100
+    c.v[0][17] = 1.0
+    c.fill()
+    got = c.upload().attend(queue)
+    c.check(got)
+    want, tol = c.expect()
+    assert (want - 1.0 > 10 * tol).mean() > 0.99 and (tol > 0).all()
