@@ -96,3 +96,24 @@ def test_small_weights_count(queue, kind, n):
     c.check(got)
     want, tol = c.expect()
     assert (want - 1.0 > 10 * tol).mean() > 0.99 and (tol > 0).all()
+
+
+@pytest.mark.parametrize("form", ["few", "many"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", [mil.KV_INT8, mil.KV_Q4])
+def test_scales_at_multiples_of_8_bytes(monkeypatch, queue, kind, D, form):
+    case, columns = (FEW[D], 0) if form == "few" else MANY[D, 4 if D == 64 else 2]
+    monkeypatch.setattr(Cache, "columns", columns)
+    c = Cache(kind, page=16, seed=65, **case).upload()
+    held = []
+    for name in "kv":
+        scales = c.scale[name].reshape(-1)
+        held.append(mil.Buffer.from_host(np.concatenate([np.full(4, 0x7e00, np.uint16), scales])))
+        assert held[-1].ptr % 16 == 0
+    c.cache = mil.KVCache(kind, c.n_pages, 16, c.kv, D, c.dev["k"], c.dev["v"], *(b.ptr + 8 for b in held))
+    c.check(c.attend(queue))
+    at = c.dev_qkv.ptr + 2 * c.heads * D
+    assert mil.kv_write(queue, c.cache, c.batch, at, at + 2 * c.kv * D, c.ld, c.ld)
+    queue.finish()
+    for name, b in zip("kv", held):
+        assert np.array_equal(b.read(np.uint16, (4 + c.scale[name].size,))[4:], c.scale[name].reshape(-1))
