@@ -66,7 +66,7 @@ constexpr size_t flash_lds(int D, int KS) { return 2 * KS * tile_bytes(D); }
 // tile), the exponentials and the waits between the phases overlap only across wavefronts.  Counters at 2048 rows,
 // 14 heads over 2: matrix cores busy 17 % of the SIMD-cycles, LDS 52 % of the CU-cycles (38 % of that bank conflicts).
 // us per launch, launches back to back: 433 in the reference's order (attention_group_kernel), 22.7 here (0.33
-// PFLOP/s, causal half counted; a large matrix product reaches 1.5); 300 rows at position 900: 96 -> 11.4.
+// PFLOP/s, causal half counted; a large fp16 product x W^T reaches 1.5); 300 rows at position 900: 96 -> 11.4.
 // Requesting tiles two ahead, forming the next tile's scores under the current tile's exponentials, and two sets
 // per wavefront were no faster.
 template <int D, int WAVES, int KS>

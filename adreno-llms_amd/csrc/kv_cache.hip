@@ -70,7 +70,8 @@ __device__ __forceinline__ uint32_t max_of(uint32_t m) {
 // A wavefront has one row of keys or values (blockIdx.y), 512 of its elements at a time, 8 to a lane.  Bound by bytes where there
 // are many rows, by the chain of loads to a row's place (q_start, kv_len, pages) where there are few.  A thread for every 8
 // elements that looked its place up by itself took 42 us to read 6 Q4 conversations of up to 8000 (102 MB); so it is 26.5, 3.85 TB/s.
-// 2048 rows of 8 x 128 written as int8 and read back, 25 MB: 9.7 us for the two launches, 2.6 TB/s; 7 rows written: 2.5 us.
+// 2048 rows of 8 x 128 written as int8 and read back, 25 MB: 10.0 us for the two launches, 2.5 TB/s; in fp16 / int8 / Q4 written 5.2 / 5.5 / 4.9,
+// read 5.7 / 4.9 / 5.1; 31800 such rows read back 53 / 45 / 45 us, 4.9 / 4.4 / 3.7 TB/s; 7 rows written: 2.5 us.
 template <int KIND, int D>
 __global__ __launch_bounds__(kThreads) void kv_write_kernel(const PagedArgs a, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                             const int64_t ld_k, const int64_t ld_v) {

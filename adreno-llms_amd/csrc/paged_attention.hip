@@ -338,7 +338,10 @@ __device__ __forceinline__ bool odd_values(const Tile<KIND, D, PAGES16>& t, cons
 // What bounds it: memory where the cache is long (16 rows make 32 operations per byte of fp16, 1/8 of what the matrix cores take for
 // each that memory gives): 656 MB of fp16 in 135.8 us, 4.84 TB/s, a large copy 4.93.  Where it is short, 7 us that do not depend on
 // its length: launch 1.4, planning 0.9 to 1.3, the first page's number 0.6, parts to the workspace 0.8 to 1.1, arrival 0.4, the
-// merge 1.6 to 2: 32 conversations of 14 heads over 2, 14 MB of int8, 8.7 us; 27 MB of Q4, 17 conversations, 14.9.
+// merge 1.6 to 2: 32 conversations of 14 heads over 2, 14 MB of int8, 8.7 us; 27 MB of Q4, 61 conversations, 15.0.  In Q4 codes to numbers
+// keep the vector units busy 63 % of the time of a long step (fp16 8 %): 549 MB in 140 us, 3.9 TB/s; 545 MB of int8 4.65 TB/s.
+// Planning looks at 64 sequences at a time, each a trip to memory: tokens behind 200 positions of 14 heads over 2, 32 / 64 / 65 / 128 sequences
+// 5.5 / 5.6 / 6.1 / 7.0 us, and then with the bytes 256 / 512 / 1024 / 4096 13 / 27 / 65 / 339 (floors 5 / 11 / 21 / 85).
 //
 // Four wavefronts to a block; with eight those 32 conversations took 15.6 us for 9.9 (then).  A tile's memory in flight per wavefront is what its
 // registers hold, so width 64 asks for four blocks to a compute unit and 128 for two.  Width 64 in fp16 with pages that end inside a
@@ -703,6 +706,10 @@ constexpr int chunk_lds_all(int D, int KS) { return KS * (chunk_lds(D) + 2 * kCh
 constexpr int meet_floats(int D, int RW) { return RW * 64 * (D / 2 + 3); }         // of a slice's sums
 __device__ __forceinline__ constexpr int twist(int row) { return (row & 3) * 2 + (row >> 2 & 1); }
 
+// Dear: a row takes its keys one to a lane and its values one after the other.  A prompt of 2048 rows of 14 heads over 2 with one NaN among
+// the values of a head's first, middle and last position 0.5, 3.2 and 5.5 ms instead of 0.03, 4096 rows of 32 over 8 0.8, 26 and 50 ms
+// instead of 0.23 (single launches).
+//
 // Row `q` (fp16) of a query at position pos against tiles first .. last - 1 of a sequence, one key to a lane: where an infinity or a
 // NaN in a place that some row must not see keeps the row off the matrix cores.  Leaves elements lane, lane + 64, .. of the sum of the
 // weighted values, and the sums' base.

@@ -114,7 +114,8 @@ constexpr PagedLaunch slices_launch(const AttentionSize& a, const Room& room, in
 // of parts in memory, 33 KB per block.  Measured, us, width 64, 128 rows / 64 in four slices: 2048 rows of 14 heads over 2 (224
 // sets) 28.5 / 33.5: blocks enough; 676 of 16 over 8 in a window of 435 (88 sets) 19.4 / 14.9; 14 sequences of 9 over 3 in a window
 // of 137 21.4 / 16.6.
-// Width 128, 128 rows / in two slices: 17 conversations of 32 heads over 8 (208 sets) 125 / 100, 14 of 16 over 8 90 / 74; 1024 sets 109 / -.
+// Width 128, 128 rows / in two slices: 17 conversations of 32 heads over 8 (320 sets as counted here, 208 there are) 125 / 100, 14 of 16 over
+// 8 90 / 74; 1024 sets 109 / -.
 //
 // Beside one block per set, as many as fill the chip, and at least half as many as it has CUs: sequences of other lengths need parts
 // to be of one length.  None at least / half / one per CU: 32 sequences of 14 tokens to 3000 35.1 / 22.3 / 29.7; 14 of 64 tokens to 4000
@@ -143,6 +144,8 @@ constexpr PagedLaunch chunk_launch(const AttentionSize& a, const Room& room, int
 //   16 heads of their own, width 128: 512 sets at 600 (38) 15.8 / 20.8, 1024 (76) 23.8 / 21.8.
 //   300 tokens of 14 heads behind 900, int8 12.8 / 14.0.
 //   Up to 32 rows, at any length: 8 sequences of 28 rows at 2000 8.6 / 13.1; 32 rows, width 128, at 2000 11.9 / 19.5.
+// The work alone does not tell it all: few sets behind many positions (28 and 64 at 16000) are sent to the slower side, as the kernel for many
+// rows adds the parts of a set one after another.
 // The host knows the lengths' bound alone, the page table's width (or the window): a table much wider than its sequences are
 // long moves them to the kernel for many rows sooner.
 constexpr int kFew = 32, kEachCu = 48;

@@ -77,7 +77,8 @@ int mi_kv_read(void* stream, const mi_kv_cache* cache, const mi_kv_batch* batch,
  * and, with window > 0, also j > p - window or j < sinks (window <= 0: sinks mean nothing).  scale: what products are multiplied
  * with before the softmax, usually 1 / sqrt(head_dim); greater than 0, at most 65504.  A row that sees nothing (and one whose
  * scores are all -infinity) is written as zeros.  What a masked position holds, NaN and infinities included, does
- * not touch the row (next to such values a row may be summed in another order, with other roundings).  out may not overlap q or the cache. */
+ * not touch the row (next to such values a row may be summed in another order, with other roundings, and a chunk of many rows takes a
+ * hundred times as long).  Scores may be of any size that fp32 holds.  out may not overlap q or the cache. */
 typedef struct mi_attention_call {
     const mi_kv_cache* cache;
     const mi_kv_batch* batch;
