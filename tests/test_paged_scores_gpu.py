@@ -88,3 +88,31 @@ def test_scores_of_minus_infinity_alone_give_zeros(monkeypatch, queue, odd, form
     c.v[0][::3, :, 7] = odd
     c.fill()
     assert (c.upload().attend(queue).view(np.uint16) & 0x7fff == 0).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("kind", KINDS)
+def test_heads_of_either_kind_side_by_side(monkeypatch, queue, kind, form):
+    """One head of a group with scores in the 10^8s, the other with ordinary ones: rows of one matrix, each as by itself."""
+    n, m, columns = form
+    monkeypatch.setattr(Cache, "columns", columns)
+    c = Cache(kind, 4, 2, 64, 16, [m], [n], seed=33)
+    for head in (0, 2):
+        c.qkv[:, head * 64:head * 64 + 64] = 0
+        c.qkv[:, head * 64] = 3 * 2.0 ** 13
+    for b in c.k:
+        b[:, :, 0] = 7 * 2.0 ** 9                         # (its products with the far heads' queries: 21 2^22)
+        b[:, :, 1:] = np.clip(b[:, :, 1:], -3, 3)
+    for head in (1, 3):
+        c.qkv[:, head * 64] = 0
+    if kind != mil.KV_F16:                               # (a scale for so large an element leaves the others 0: ordinary scores are)
+        c.k[0][:, :, 1:] = 0
+    c.fill()
+    got = c.upload().attend(queue, scale=7.3)
+    v = _values(c)
+    want, mean = (np.cumsum(x, 0)[m - n:] / np.arange(m - n + 1, m + 1)[:, None, None] for x in (v, np.abs(v)))
+    far = got[:, [0, 2]].astype(np.float64)
+    tol = 2.0 ** -11 * np.abs(want) + (m + 2) * 2.0 ** -24 * mean + 2.0 ** -25
+    assert (np.abs(far - want) <= tol).all()
+    want, tol = c.expect(scale=7.3)
+    assert (np.abs(got[:n].astype(np.float64) - want) <= tol)[:, [1, 3]].all()
