@@ -69,6 +69,11 @@ _SIGNATURES = {
     "mi_kv_write": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i]),
     "mi_kv_read": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i]),
     "mi_attention": (_i, [_vp, _vp]),
+    "mi_rope": (_i, [_vp, _vp]),
+    "mi_attention_tree": (_i, [_vp, _vp, _vp]),
+    "mi_kv_keep": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp]),
+    "mi_kv_reorder": (_i, [_vp, _vp, _i, _vp]),
+    "mi_beam_select": (_i, [_vp, _vp]),
     "mi_argmax_f16": (_i, [_vp, _vp, _i, _i, _vp]),
     "mi_linear_argmax": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
     "mi_linear_argmax_static": (_i, [_vp, _i, _i, _vp, _vp, _vp, _i, _vp]),
@@ -451,6 +456,92 @@ def kv_read(queue, cache, batch, k_out, v_out, ld_k=0, ld_v=0):
 def attention(queue, call):
     """Attention of the new tokens over the cache (mi_attention)."""
     return bool(lib().mi_attention(_q(queue), call._at))
+
+
+class RopeCall(C.Structure):
+    """mi_rope_call: a prepared call of rope().  Rows of n_heads heads q -> q_out and of n_kv_heads k -> k_out; ld_*: elements from row
+    to row (0: the heads' own); inv_freq float32 [rot_dim / 2], position int32 [n_axes, n_tokens] in device memory; axis: of each
+    pair the number of its axis (None: one axis)."""
+    _fields_ = [(n, _vp) for n in ("q", "k", "q_out", "k_out", "inv_freq", "position", "axis")] + \
+               [(n, _i) for n in ("ld_q", "ld_k", "ld_q_out", "ld_k_out", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "rot_dim",
+                                  "n_axes", "interleaved")]
+
+    def __init__(self, n_tokens, n_heads, n_kv_heads, head_dim, rot_dim, inv_freq, position, q=None, q_out=None, k=None, k_out=None,
+                 ld_q=0, ld_k=0, ld_q_out=0, ld_k_out=0, axis=None, n_axes=0, interleaved=False):
+        wide, narrow = n_heads * head_dim, n_kv_heads * head_dim
+        axes = None if axis is None else (C.c_ubyte * max(len(axis), 1))(*axis)
+        if axis is not None and len(axis) != rot_dim // 2:
+            raise ValueError(f"an axis for each of {rot_dim // 2} pairs, got {len(axis)}")
+        super().__init__(_h(q), _h(k), _h(q_out), _h(k_out), _h(inv_freq), _h(position), None if axes is None else C.addressof(axes),
+                         ld_q or wide, ld_k or narrow, ld_q_out or wide, ld_k_out or narrow, n_tokens, n_heads, n_kv_heads, head_dim,
+                         rot_dim, n_axes or (1 if not axis else max(axis) + 1), int(interleaved))
+        self._keep, self._at = (q, k, q_out, k_out, inv_freq, position, axes), C.addressof(self)
+
+
+def rope(queue, call):
+    """Rotary positions of new rows' queries and keys (mi_rope)."""
+    return bool(lib().mi_rope(_q(queue), call._at))
+
+
+class TreeMask(C.Structure):
+    """mi_tree_mask: which of the call's new rows each of them sees, bits [n_tokens, words] of 32, and (with a window) the rows' places in
+    their texts, int32 [n_tokens]; device memory."""
+    _fields_ = [("seen", _vp), ("position", _vp), ("words", _i)]
+
+    def __init__(self, seen, words, position=None):
+        super().__init__(_h(seen), _h(position), words)
+        self._keep, self._at = (seen, position), C.addressof(self)
+
+
+def attention_tree(queue, call, tree):
+    """Attention of drafted tokens over the cache and their ancestors among themselves (mi_attention_tree)."""
+    return bool(lib().mi_attention_tree(_q(queue), call._at, tree._at))
+
+
+class KVCaches:
+    """The caches of several layers, for kv_keep() and kv_reorder()."""
+
+    def __init__(self, caches):
+        self.n, self.of = len(caches), (KVCache * max(len(caches), 1))(*caches)
+        self._keep, self._at = caches, C.addressof(self.of)
+
+
+def kv_keep(queue, caches, batch, keep, kept, new_len=None):
+    """Accepted rows of every sequence move together behind its earlier ones, in all caches (mi_kv_keep)."""
+    return bool(lib().mi_kv_keep(_q(queue), caches._at, caches.n, batch._at, _h(keep), _h(kept), _h(new_len)))
+
+
+class ReorderCall(C.Structure):
+    """mi_kv_reorder_call: a prepared call of kv_reorder(); int32 in device memory: kv_len, source, fresh, new_len [n_seqs], pages, new_pages
+    [n_seqs, max_pages]."""
+    _fields_ = [(n, _vp) for n in ("kv_len", "pages", "source", "fresh", "new_len", "new_pages")] + [("n_seqs", _i), ("max_pages", _i)]
+
+    def __init__(self, n_seqs, max_pages, kv_len, pages, source, fresh, new_len, new_pages):
+        held = (kv_len, pages, source, fresh, new_len, new_pages)
+        super().__init__(*map(_h, held), n_seqs, max_pages)
+        self._keep, self._at = held, C.addressof(self)
+
+
+def kv_reorder(queue, caches, call):
+    """Every sequence goes on as a copy of another (mi_kv_reorder)."""
+    return bool(lib().mi_kv_reorder(_q(queue), caches._at, caches.n, call._at))
+
+
+class BeamCall(C.Structure):
+    """mi_beam_call: a prepared call of beam_select().  logits fp16 [n_groups * beams, ld], score float32 [n_groups * beams]; out_score
+    (float32), out_token, out_row (int32) [n_groups, n_out]."""
+    _fields_ = [(n, _vp) for n in ("logits", "score", "out_score", "out_token", "out_row")] + \
+               [(n, _i) for n in ("ld", "n_groups", "beams", "vocab", "n_out")]
+
+    def __init__(self, n_groups, beams, vocab, n_out, logits, score, out_score, out_token, out_row, ld=0):
+        held = (logits, score, out_score, out_token, out_row)
+        super().__init__(*map(_h, held), ld or vocab, n_groups, beams, vocab, n_out)
+        self._keep, self._at = held, C.addressof(self)
+
+
+def beam_select(queue, call):
+    """The best continuations of every group's beams (mi_beam_select)."""
+    return bool(lib().mi_beam_select(_q(queue), call._at))
 
 
 # ------------------------------------------------------------------- offline tools

@@ -295,32 +295,29 @@ extern "C" int mi_kv_read(void* stream, const mi_kv_cache* cache, const mi_kv_ba
     return MI_KV_LAUNCH(kv_read_kernel, static_cast<uint16_t*>(k), static_cast<uint16_t*>(v));
 }
 
-extern "C" int mi_attention(void* stream, const mi_attention_call* call) {
-    if (!call) {
-        MI_ERROR_FMT("mi_attention: null call");
-        return 0;
-    }
-    const mi_attention_call& c = *call;
+namespace {
+
+// Checks a call of mi_attention, or of `who` which goes by the same, and makes the kernels' form.  1: to be launched, 0: nothing to do, -1:
+// refused.
+int attention_args(const char* who, const mi_attention_call& c, AttentionArgs& a) {
     PagedArgs p;
-    if (!paged_args("mi_attention", c.cache, c.batch, &p)) return 0;
+    if (!paged_args(who, c.cache, c.batch, &p)) return -1;
     const int64_t width = static_cast<int64_t>(c.n_heads) * c.cache->head_dim;
     if (c.n_heads < 1 || c.n_heads % p.n_kv_heads || !c.q || !c.out || c.ld_q < width || c.ld_out < width ||
         reinterpret_cast<uintptr_t>(c.q) % 2 || reinterpret_cast<uintptr_t>(c.out) % 2) {
-        MI_ERROR_FMT("mi_attention: bad argument (n_heads=%d over %d q=%p ld_q=%d out=%p ld_out=%d)", c.n_heads, p.n_kv_heads, c.q, c.ld_q,
+        MI_ERROR_FMT("%s: bad argument (n_heads=%d over %d q=%p ld_q=%d out=%p ld_out=%d)", who, c.n_heads, p.n_kv_heads, c.q, c.ld_q,
                      c.out, c.ld_out);
-        return 0;
+        return -1;
     }
     if (!(c.scale > 0.0f && c.scale <= 65504.0f) || c.sinks < 0) {
-        MI_ERROR_FMT("mi_attention: bad argument (scale=%g, window=%d, sinks=%d)", static_cast<double>(c.scale), c.window, c.sinks);
-        return 0;
+        MI_ERROR_FMT("%s: bad argument (scale=%g, window=%d, sinks=%d)", who, static_cast<double>(c.scale), c.window, c.sinks);
+        return -1;
     }
-    if (p.n_seqs == 0 || p.n_tokens == 0) return 1;
+    if (p.n_seqs == 0 || p.n_tokens == 0) return 0;
     if (static_cast<int64_t>(p.n_tokens) * c.n_heads > 0x3fffffff) {
-        MI_ERROR_FMT("mi_attention: %d rows of %d heads are more than a launch counts", p.n_tokens, c.n_heads);
-        return 0;
+        MI_ERROR_FMT("%s: %d rows of %d heads are more than a launch counts", who, p.n_tokens, c.n_heads);
+        return -1;
     }
-    if (!ensure_init()) return 0;
-    AttentionArgs a{};
     a.p = p;
     a.q = static_cast<const uint16_t*>(c.q);
     a.out = static_cast<uint16_t*>(c.out);
@@ -333,6 +330,48 @@ extern "C" int mi_attention(void* stream, const mi_attention_call* call) {
     a.window = c.window;
     a.sinks = c.sinks;
     a.scale = c.scale;
+    return 1;
+}
+
+}  // namespace
+
+extern "C" int mi_attention(void* stream, const mi_attention_call* call) {
+    if (!call) {
+        MI_ERROR_FMT("mi_attention: null call");
+        return 0;
+    }
+    AttentionArgs a{};
+    const int todo = attention_args("mi_attention", *call, a);
+    if (todo <= 0) return todo == 0;
+    if (!ensure_init()) return 0;
     const auto s = static_cast<hipStream_t>(stream);
     return launch_paged_attention(s, a, stream_room(s)) ? 1 : 0;
+}
+
+extern "C" int mi_attention_tree(void* stream, const mi_attention_call* call, const mi_tree_mask* tree) {
+    if (!call || !tree) {
+        MI_ERROR_FMT("mi_attention_tree: null call or tree");
+        return 0;
+    }
+    TreeArgs a{};
+    const int todo = attention_args("mi_attention_tree", *call, a);
+    if (todo < 0) return 0;
+    if (tree->words < 1 || tree->words > 65536) {
+        MI_ERROR_FMT("mi_attention_tree: bad argument (words=%d)", tree->words);
+        return 0;
+    }
+    if (todo == 0) return 1;
+    const bool windowed = call->window > 0;
+    if (!tree->seen || reinterpret_cast<uintptr_t>(tree->seen) % 4 || (windowed && !tree->position) ||
+        reinterpret_cast<uintptr_t>(tree->position) % 4) {
+        MI_ERROR_FMT("mi_attention_tree: bad argument (seen=%p position=%p window=%d)", static_cast<const void*>(tree->seen),
+                     static_cast<const void*>(tree->position), call->window);
+        return 0;
+    }
+    if (!ensure_init()) return 0;
+    a.seen = tree->seen;
+    a.position = tree->position;
+    a.words = tree->words;
+    const auto s = static_cast<hipStream_t>(stream);
+    return launch_paged_tree(s, a, stream_room(s)) ? 1 : 0;
 }

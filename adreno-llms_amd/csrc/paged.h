@@ -27,7 +27,7 @@ __device__ __forceinline__ int64_t row_number(const PagedArgs& a, int page, int 
            static_cast<uint32_t>(head * a.page.d + slot);
 }
 
-// paged_attention.hip
+// paged_kernels.h: of mi_attention, and (TreeArgs) of mi_attention_tree
 struct AttentionArgs {
     PagedArgs p;
     const uint16_t* q;
@@ -37,6 +37,12 @@ struct AttentionArgs {
     int window, sinks;
     float scale;
 };
-bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, const StreamRoom& room);
+struct TreeArgs : AttentionArgs {
+    const uint32_t* seen;                     // [n_tokens][words]
+    const int* position;                      // [n_tokens], of calls with a window
+    int words;
+};
+bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, const StreamRoom& room);     // paged_attention.hip
+bool launch_paged_tree(hipStream_t s, const TreeArgs& a, const StreamRoom& room);               // paged_tree.hip
 
 }  // namespace mi

@@ -94,6 +94,73 @@ typedef struct mi_attention_call {
  * before it meets the values.  The same call on the same data gives the same bits. */
 int mi_attention(void* stream, const mi_attention_call* call);
 
+/* Rotary positions of new rows, between the projections and the cache.  Of each head of head_dim elements the first rot_dim are
+ * pairs (x, y): elements i and i + rot_dim / 2, or with `interleaved` not 0 2 i and 2 i + 1, i = 0 .. rot_dim / 2 - 1, and become
+ *   (x cos a - y sin a, y cos a + x sin a),  a = position[axis of i][row] * inv_freq[i];
+ * the elements behind them are copied.  One position per row and axis: a text has one axis, pictures and films have their rows' time, line
+ * and column.  A negative position turns the other way, by which keys can be turned back.
+ *   q, q_out    rows of n_heads heads, ld_q and ld_q_out elements apart; k, k_out: of n_kv_heads, the same (either may have 0 heads and be
+ *               null).  fp16, 2-byte aligned.  An output may be its own input, with the same ld; else outputs overlap nothing.
+ *   position    int32 [n_axes][n_tokens], inv_freq fp32 [rot_dim / 2]: device memory.
+ *   axis        host memory, read during the call: of each i the number of its axis; null: all 0.
+ * head_dim even, up to 256; rot_dim even, 0 to head_dim; n_axes 1 to 4.  The angle is taken in 64 bits and cosine and sine to fp32's last
+ * bits at any position; an output is rounded to fp16 once.  The reference has one axis, the halves' pairs and fp16 tables
+ * (QW/kernels/rope.cl, QW/src/layers/attention.cpp:133-172), as mi_decoder_step keeps them. */
+typedef struct mi_rope_call {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const float* inv_freq;
+    const int* position;
+    const unsigned char* axis;
+    int ld_q, ld_k, ld_q_out, ld_k_out;
+    int n_tokens, n_heads, n_kv_heads, head_dim, rot_dim, n_axes, interleaved;
+} mi_rope_call;
+int mi_rope(void* stream, const mi_rope_call* call);
+
+/* ---- several continuations of a sequence ----------------------------------------------------------------------
+ *
+ * A host that has tokens drafted ahead, or keeps several beams, has more than one continuation of a sequence in the cache. */
+
+/* Attention of drafted tokens.  The new rows of a sequence (mi_kv_write has put their keys and values behind the others, in the
+ * order of the rows) are no text one after the other but, say, a tree: row i sees all positions before the sequence's new ones,
+ * and its new row j if bit j % 32 of seen[row * words + j / 32] is set, `row` the number of i in the batch; its own bit is set by
+ * the caller too.  Bits of rows that the sequence does not have count for nothing, rows past 32 * words are seen by none.
+ * With a window the earlier positions j are those with j > p - window or j < sinks, p = position[row] being the row's place in its
+ * text (as for mi_rope; taken as no less than the number of earlier positions and less than kv_len); the bits alone
+ * decide among new rows.  seen [n_tokens][words] and position [n_tokens]: device memory, 4-byte aligned; position may be null where
+ * there is no window.  words 1 to 65536.  All else as mi_attention, whose kernels these are. */
+typedef struct mi_tree_mask {
+    const unsigned* seen;
+    const int* position;
+    int words;
+} mi_tree_mask;
+int mi_attention_tree(void* stream, const mi_attention_call* call, const mi_tree_mask* tree);
+
+/* Of the new rows of every sequence, accepted drafts stay and move together.  Of sequence b, with n_b new rows behind `before` = kv_len[b] -
+ * n_b earlier positions, the rows numbered keep[q_start[b] + i], i = 0 .. kept[b] - 1, ascending, each of 0 .. n_b - 1, become
+ * positions before + i, in every cache of `caches`; what the other positions hold is left as it is.  new_len[b] = before + kept[b] (kept
+ * taken as within 0 .. n_b; less than 0 counts as 0) unless new_len is null; it may be neither kv_len nor kept.
+ * caches: n_caches of them, the layers of a model say, which differ in their pools alone.  keep [n_tokens] (what lies behind a
+ * sequence's kept ones is not read), kept [n_seqs], new_len [n_seqs]: device memory, 4-byte aligned.  Rows move as they are stored.  A row
+ * or a place that is not in the cache, or a number out of range, moves nothing.  Where numbers do not ascend it is not said
+ * which rows end up where, but no other positions are touched.  No two sequences of a call share a page that holds a new row. */
+int mi_kv_keep(void* stream, const mi_kv_cache* caches, int n_caches, const mi_kv_batch* batch, const int* keep, const int* kept,
+               int* new_len);
+
+/* Sequences go on as copies of others: beam search's reordering.  Sequence b becomes what sequence f = source[b] is: new_len[b] = kv_len[f];
+ * new_pages[b] is pages[f], up to the pages that kv_len[f] positions need, -1 behind them, but for a last page that is not full: its
+ * kv_len[f] % page_size rows are copied, in every cache of `caches`, to page fresh[b], which takes its place (f = b keeps its own and fresh[b] is
+ * not used).  Full pages are shared from then on, which the host counts.  source[b] outside 0 .. n_seqs - 1: new_len[b] = 0, all
+ * pages -1.  kv_len[f] beyond the table, or a page (old or fresh) that is not in the pool: the number is passed on, nothing is copied.
+ * A fresh page is nobody's: neither in `pages` nor twice in `fresh` among those that are used.  kv_len, source, fresh, new_len
+ * [n_seqs], pages, new_pages [n_seqs][max_pages]: device memory, 4-byte aligned; new_len and new_pages overlap none of the others. */
+typedef struct mi_kv_reorder_call {
+    const int *kv_len, *pages, *source, *fresh;
+    int *new_len, *new_pages;
+    int n_seqs, max_pages;
+} mi_kv_reorder_call;
+int mi_kv_reorder(void* stream, const mi_kv_cache* caches, int n_caches, const mi_kv_reorder_call* call);
+
 #ifdef __cplusplus
 }
 #endif

@@ -143,6 +143,27 @@ int mi_linear_argmax(void* stream, int N, int K, const void* x, const void* W, v
 int mi_linear_argmax_static(void* stream, int N, int K, const void* x, const void* W, void* logits,
                             int num_partials, void* token_out);
 
+/* Beam search's choice of continuations, on the device.  n_groups searches with `beams` beams each: rows g * beams .. g * beams + beams - 1
+ * of logits (fp16 [n_groups * beams], ld elements apart, `vocab` of them) and score (fp32, the sum of log probabilities so far) are group
+ * g's.  Its n_out best continuations are left, best first, in out_score, out_token and out_row [n_groups][n_out]: token t of row r counts
+ *   score[r] + logits[r][t] - log sum_u exp logits[r][u],
+ * compared in 64 bits and left as fp32; among equals the lowest row, then the lowest token.  -infinity is a logit that is never chosen (a
+ * token that a grammar forbids); a row whose score is not finite (a beam that is not there, the others of a first step), whose
+ * logits are all -infinity, or that holds a NaN or +infinity is never chosen from.  Where fewer than n_out are left the others are
+ * -infinity, -1, -1.  out_row is a number of all rows, as mi_kv_reorder takes it.  With n_out = 2 * beams a host has enough whichever
+ * of them end.  The reference decodes greedily or samples; it has no beams.
+ * beams and n_out 1 to 64, vocab up to MI_BEAM_MAX_VOCAB.  Two launches on a stream of mi_stream_create or the null stream, whose
+ * workspace holds the rows' sums and maxima in between; on any other stream one launch, slower.  Nothing is allocated or waited for. */
+#define MI_BEAM_MAX_VOCAB (1 << 21)
+typedef struct mi_beam_call {
+    const void* logits;
+    const float* score;
+    float* out_score;
+    int *out_token, *out_row;
+    int ld, n_groups, beams, vocab, n_out;
+} mi_beam_call;
+int mi_beam_select(void* stream, const mi_beam_call* call);
+
 /* One call of mi_linear, for mi_linear_batch. */
 typedef struct mi_linear_call {
     int M, N, K;

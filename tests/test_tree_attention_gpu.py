@@ -1,0 +1,161 @@
+"""mi_attention_tree against a plain evaluation in 64 bits (tree_lib.TreeCache.expect).  Everything that no row may see is NaN in
+these caches; a chain of drafts is what mi_attention makes of the same rows."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from helpers import mil
+from paged_lib import Cache
+from tree_lib import TreeCache, ancestors
+
+pytestmark = pytest.mark.gpu
+KINDS = [mil.KV_F16, mil.KV_INT8, mil.KV_Q4]
+
+
+@pytest.fixture(scope="module")
+def queue():
+    assert mil.lib().mi_init(0) == 1
+    return mil.Queue()
+
+
+@pytest.fixture(autouse=True, params=[0, 2 ** 20], ids=["tight", "wide"])
+def columns(request, monkeypatch):
+    """Small batches run on the kernel for few rows; under a page table for a million positions every sequence of more than 32 rows
+    runs on the one for many."""
+    monkeypatch.setattr(Cache, "columns", request.param)
+    return request.param
+
+
+CASES = [
+    dict(heads=14, kv_heads=2, D=64, page=16, lengths=[40], new=[16]),
+    dict(heads=14, kv_heads=2, D=64, page=16, lengths=[16], new=[16]),                       # nothing but drafts
+    dict(heads=9, kv_heads=3, D=64, page=64, lengths=[1, 5, 64, 65, 0, 300], new=[1, 4, 33, 31, 0, 32], pad=3),
+    dict(heads=8, kv_heads=8, D=128, page=1, lengths=[130, 17], new=[40, 17]),
+    dict(heads=32, kv_heads=8, D=128, page=48, lengths=[700, 97, 48, 49], new=[64, 37, 1, 24]),
+    dict(heads=15, kv_heads=5, D=64, page=100, lengths=[1500, 199, 101], new=[100, 99, 3], gap=3),
+    dict(heads=8, kv_heads=1, D=128, page=32, lengths=[460, 333], new=[130, 129]),
+    dict(heads=4, kv_heads=1, D=64, page=2048, lengths=[5000], new=[65], spare=0),
+]
+
+
+@pytest.mark.parametrize("case", CASES)
+@pytest.mark.parametrize("kind", KINDS)
+def test_against_64_bits(queue, kind, case):
+    c = TreeCache(kind, seed=1, **case).upload()
+    c.check(c.attend(queue))
+    c.check(c.attend(queue, ld_out=c.heads * c.D + 5), what="rows apart")
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (33, 0), (100, 37), (2 ** 31 - 1, 2 ** 31 - 1)])
+@pytest.mark.parametrize("case", [CASES[0], CASES[2], CASES[4], CASES[5]])
+@pytest.mark.parametrize("kind", [mil.KV_F16, mil.KV_Q4])
+def test_windows(queue, kind, case, window, sinks):
+    c = TreeCache(kind, seed=2, **case).upload()
+    c.check(c.attend(queue, window=window, sinks=sinks), window, sinks)
+
+
+@pytest.mark.parametrize("case", [CASES[2], CASES[5], CASES[6]])
+@pytest.mark.parametrize("kind", [mil.KV_F16, mil.KV_INT8])
+def test_any_bits(queue, kind, case):
+    """Masks that are no trees: later rows, not the row's own, none at all (with nothing before: zeros)."""
+    rng = np.random.default_rng(3)
+    masks = [rng.random((n, n)) < 0.3 for n in case["new"]]
+    for m in masks:
+        m[::5] = False
+    c = TreeCache(kind, seed=3, masks=masks, **case).upload()
+    c.check(c.attend(queue))
+
+
+def test_rows_that_see_nothing(queue):
+    n = 40
+    masks = [np.zeros((n, n), bool)]
+    masks[0][3, 7] = True
+    c = TreeCache(mil.KV_F16, 14, 2, 64, 16, [n], [n], masks=masks).upload()
+    got = c.attend(queue)
+    c.check(got)
+    assert (got[[r for r in range(n) if r != 3]] == 0).all()
+
+
+@pytest.mark.parametrize("words", [1, 2, 3, 7])
+def test_words(queue, words):
+    """Rows past the words are seen by none; words past the rows count for nothing."""
+    c = TreeCache(mil.KV_F16, 14, 2, 64, 16, [300, 80], [70, 33], words=words, seed=4).upload()
+    c.check(c.attend(queue))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("case", [CASES[0], CASES[4], CASES[6]])
+def test_a_chain_is_a_text(queue, kind, case):
+    """Bits of a lower triangle: what mi_attention has to give."""
+    masks = [np.tril(np.ones((n, n), bool)) for n in case["new"]]
+    c = TreeCache(kind, seed=5, masks=masks, **case).upload()
+    plain = Cache.__new__(Cache)
+    plain.__dict__ = c.__dict__
+    plain.check(c.attend(queue))
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("kind", [mil.KV_F16, mil.KV_INT8])
+def test_infinities_and_nans_of_drafts_that_are_not_seen(queue, kind, bad):
+    """Every odd draft's keys and values are NaN or infinite; the even ones do not see them."""
+    n, m = 48, 200
+    masks = [np.tril(np.ones((n, n), bool))]
+    masks[0][::2, 1::2] = False
+    c = TreeCache(kind, 14, 2, 64, 16, [m], [n], masks=masks, seed=6)
+    c.k[0][m - n + 1::2] = bad
+    c.v[0][m - n + 1::2] = bad
+    c.fill()
+    got = c.upload().attend(queue)
+    masks[0][1::2] = False                                # (the odd ones are not looked at)
+    c.check(got, rows=slice(0, n, 2))
+
+
+def test_repeated_and_captured(queue):
+    """The same bits again, and from a graph that follows lengths and bits on the device."""
+    c = TreeCache(mil.KV_INT8, 14, 2, 64, 64, [900, 3000, 64], [24, 17, 9], seed=7).upload()
+    first = c.attend(queue)
+    assert (c.attend(queue).view(np.uint16) == first.view(np.uint16)).all()
+    width = c.heads * c.D
+    out = mil.Buffer.from_host(np.zeros((c.rows, width), np.uint16))
+    seen = mil.Buffer.from_host(np.ascontiguousarray(c.seen))
+    call = mil.AttentionCall(c.cache, c.batch, c.heads, c.dev_qkv, out, ld_q=c.ld)
+    mask = mil.TreeMask(seen, c.words)
+    assert mil.lib().mi_graph_begin(queue.handle)
+    assert mil.attention_tree(queue, call, mask)
+    graph = mil.lib().mi_graph_end(queue.handle)
+    assert graph
+    for turn in range(3):
+        assert mil.lib().mi_graph_launch(graph, queue.handle)
+        queue.finish()
+        got = out.read(np.float16, (c.rows, c.heads, c.D))
+        c.check(got, what=turn)
+        rng = np.random.default_rng(turn)
+        c.masks = [ancestors([-1] + [int(rng.integers(0, i)) for i in range(1, n)]) for n in c.new]
+        bits = np.zeros((c.rows, 32 * c.words), bool)
+        for b, m in enumerate(c.masks):
+            bits[c.start[b]:c.start[b] + len(m), :len(m)] = m
+        c.seen = np.packbits(bits.reshape(c.rows, c.words, 32), axis=2, bitorder="little").view(np.uint32)[..., 0]
+        seen.write(np.ascontiguousarray(c.seen))
+        queue.finish()
+    mil.lib().mi_graph_destroy(graph)
+
+
+def test_long(queue):
+    """Parts of a sequence that meet in the workspace, the drafts in the last of them."""
+    c = TreeCache(mil.KV_F16, 14, 2, 64, 16, [9000, 70], [30, 1], seed=8).upload()
+    c.check(c.attend(queue))
+
+
+def test_a_stream_without_a_workspace(queue):
+    hip = ctypes.CDLL("libamdhip64.so")
+    foreign = ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(foreign)) == 0
+    c = TreeCache(mil.KV_Q4, 14, 2, 64, 16, [3000, 70], [30, 40], seed=9).upload()
+    out = mil.Buffer.from_host(np.zeros((c.rows, c.heads * c.D), np.uint16))
+    seen = mil.Buffer.from_host(np.ascontiguousarray(c.seen))
+    call = mil.AttentionCall(c.cache, c.batch, c.heads, c.dev_qkv, out, ld_q=c.ld)
+    assert mil.attention_tree(foreign, call, mil.TreeMask(seen, c.words))
+    assert hip.hipStreamSynchronize(foreign) == 0
+    c.check(out.read(np.float16, (c.rows, c.heads, c.D)))
+    assert hip.hipStreamDestroy(foreign) == 0
