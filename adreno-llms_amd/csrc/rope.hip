@@ -49,7 +49,71 @@ __device__ __forceinline__ uint16_t* to(const RopeArgs& a, int row, int head) {
     return head < a.n_heads ? a.q_out + row * a.ld_q_out + head * a.head_dim : a.k_out + row * a.ld_k_out + (head - a.n_heads) * a.head_dim;
 }
 
-// A wavefront has a row (or a part of its heads), a lane one pair after the other.
+// A wavefront has a row (or a part of its heads), a lane 16 elements of a head at a time: 8 pairs, or 16 of those behind them.  Where all
+// rows and halves are whole pieces of 16 bytes.
+template <bool SPLIT>
+__global__ __launch_bounds__(64 * kWaves) void rope_wide_kernel(const RopeArgs a) {
+    __shared__ __attribute__((aligned(16))) float turn[kWaves][2 * kMostPairs];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int item = blockIdx.x * kWaves + wave, row = item / a.parts, part = item - row * a.parts;
+    if (row >= a.n_tokens) return;
+    const int each = a.head_dim / 16, turning = a.pairs / 8, n = a.heads * each;
+    struct Piece {
+        half8 x, y;
+        int at_x, at_y, i;                         // elements of the head; first pair, -1: none
+        uint16_t* dst;
+    };
+    auto load = [&](int z) {
+        Piece p;
+        const int head = z / each, c = z - head * each;
+        const uint16_t* const src = from(a, row, head);
+        p.dst = to(a, row, head);
+        p.i = c < turning ? 8 * c : -1;
+        p.at_x = SPLIT && c < turning ? 8 * c : 16 * c;
+        p.at_y = SPLIT && c < turning ? 8 * c + a.pairs : 16 * c + 8;
+        p.x = *reinterpret_cast<const half8*>(src + p.at_x);
+        p.y = *reinterpret_cast<const half8*>(src + p.at_y);
+        return p;
+    };
+    auto finish = [&](Piece p) {
+        if (p.i >= 0) {
+            float c[8], s[8];
+            #pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const floatx4 cs = *reinterpret_cast<const floatx4*>(&turn[wave][p.i + e]);
+                const floatx4 sn = *reinterpret_cast<const floatx4*>(&turn[wave][kMostPairs + p.i + e]);
+                #pragma unroll
+                for (int z = 0; z < 4; ++z) c[e + z] = cs[z], s[e + z] = sn[z];
+            }
+            #pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                _Float16 &x = SPLIT ? reinterpret_cast<_Float16*>(&p.x)[e] : e < 4 ? reinterpret_cast<_Float16*>(&p.x)[2 * e] : reinterpret_cast<_Float16*>(&p.y)[2 * e - 8];
+                _Float16 &y = SPLIT ? reinterpret_cast<_Float16*>(&p.y)[e] : e < 4 ? reinterpret_cast<_Float16*>(&p.x)[2 * e + 1] : reinterpret_cast<_Float16*>(&p.y)[2 * e - 7];
+                const float fx = static_cast<float>(x), fy = static_cast<float>(y);
+                x = static_cast<_Float16>(turned_x(fx, fy, c[e], s[e]));
+                y = static_cast<_Float16>(turned_y(fx, fy, c[e], s[e]));
+            }
+        }
+        *reinterpret_cast<half8*>(p.dst + p.at_x) = p.x;
+        *reinterpret_cast<half8*>(p.dst + p.at_y) = p.y;
+    };
+    // (the first two pieces are on their way while the angles are worked out)
+    const int step = 64 * a.parts, z0 = part * 64 + lane;
+    Piece now{}, next{};
+    if (z0 < n) now = load(z0);
+    if (z0 + step < n) next = load(z0 + step);
+    angles(a, row, lane, turn[wave]);
+    __builtin_amdgcn_wave_barrier();
+    for (int z = z0; z < n; z += step) {
+        Piece after{};
+        if (z + 2 * step < n) after = load(z + 2 * step);
+        finish(now);
+        now = next;
+        next = after;
+    }
+}
+
+// The same for any rows, a lane one pair after the other.
 template <bool SPLIT>
 __global__ __launch_bounds__(64 * kWaves) void rope_kernel(const RopeArgs a) {
     __shared__ float turn[kWaves][2 * kMostPairs];
@@ -143,7 +207,10 @@ extern "C" int mi_rope(void* stream, const mi_rope_call* call) {
     const auto go = [&](auto kern) {
         hipLaunchKernelGGL(kern, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream), a);
     };
-    if (c.interleaved) go(rope_kernel<false>);
-    else go(rope_kernel<true>);
+    const auto whole = [&](const void* p, int ld, int of) { return of == 0 || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0); };
+    const bool wide = c.head_dim % 16 == 0 && c.rot_dim % 16 == 0 && whole(c.q, c.ld_q, c.n_heads) && whole(c.q_out, c.ld_q_out, c.n_heads) &&
+                      whole(c.k, c.ld_k, c.n_kv_heads) && whole(c.k_out, c.ld_k_out, c.n_kv_heads);
+    if (wide) c.interleaved ? go(rope_wide_kernel<false>) : go(rope_wide_kernel<true>);
+    else c.interleaved ? go(rope_kernel<false>) : go(rope_kernel<true>);
     return MI_HIP_OK(hipGetLastError()) ? 1 : 0;
 }
