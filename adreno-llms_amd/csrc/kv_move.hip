@@ -21,9 +21,9 @@ struct Layers {
 // ---- accepted drafts --------------------------------------------------------------------------------------
 //
 // Numbers ascend, so row keep[i] >= i moves down or stays, and rows done in order never overwrite one that is still to be read.  A wavefront
-// has some 16-byte columns of a sequence's rows in one pool, all of its kept rows, as many at a time as its lanes and kAhead registers
-// take: these are all read before the first of them is written.
-constexpr int kAhead = 4;
+// has some 16-byte columns of a sequence's rows in one pool and looks up where 64 of its kept rows come from and go to, one to a lane;
+// then it moves as many at a time as its lanes and kAhead registers take: these are all read before the first of them is written.
+constexpr int kAhead = 8;
 
 struct KeepArgs {
     PagedArgs p;
@@ -49,46 +49,55 @@ __global__ __launch_bounds__(64) void kv_keep_kernel(const KeepArgs a, const Lay
     uint8_t* const pool = blockIdx.y % 2 ? pools.v : pools.k;
     uint16_t* const scales = blockIdx.y % 2 ? pools.v_scale : pools.k_scale;
     const int* const table = a.p.pages + static_cast<int64_t>(b) * a.p.max_pages;
-    const auto place = [&](int pos) {
+    const auto place = [&](int pos) {              // of head 0's row
         if (pos < 0 || pos >= a.p.cap) return static_cast<int64_t>(-1);
         const int page = divide(pos, a.p.page), number = table[page];
         if (static_cast<uint32_t>(number) >= static_cast<uint32_t>(a.p.n_pages)) return static_cast<int64_t>(-1);
-        return row_number(a.p, number, head, pos - page * a.p.page.d);
+        return row_number(a.p, number, 0, pos - page * a.p.page.d);
     };
-    for (int i0 = 0; i0 < kept; i0 += kAhead * together) {
-        int64_t src[kAhead], dst[kAhead];
-        u32x4 x[kAhead];
-        uint16_t sc[kAhead][kScales > 0 ? kScales : 1];
-        #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int i = i0 + u * together + mine;
-            src[u] = dst[u] = -1;
-            if (busy && i < kept) {
-                const int number = a.keep[s.first + i];
-                if (number != i && number >= 0 && number < s.n) {
-                    src[u] = place(s.pos + number);
-                    dst[u] = place(s.pos + i);
-                }
+    const auto of_lane = [](int64_t x, int from) {
+        return static_cast<int64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(x), from))) | static_cast<int64_t>(__shfl(static_cast<int>(x >> 32), from)) << 32;
+    };
+    for (int first = 0; first < kept; first += 64) {
+        int64_t from = -1, to = -1;                // of kept row first + lane; -1: it does not move
+        if (first + lane < kept) {
+            const int i = first + lane, number = a.keep[s.first + i];
+            if (number != i && number >= 0 && number < s.n) {
+                from = place(s.pos + number);
+                to = place(s.pos + i);
             }
-            if (src[u] < 0 || dst[u] < 0) dst[u] = -1;
+            if (from < 0) to = -1;
         }
-        #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (dst[u] >= 0) {
-                x[u] = *reinterpret_cast<const u32x4*>(pool + src[u] * row_bytes(KIND, D) + 16 * piece);
-                if constexpr (kScales > 0)
-                    if (piece == 0)
-                        for (int z = 0; z < kScales; ++z) sc[u][z] = scales[src[u] * kScales + z];
+        const int last = kept - first < 64 ? kept - first : 64;
+        for (int i0 = 0; i0 < last; i0 += kAhead * together) {
+            int64_t src[kAhead], dst[kAhead];
+            u32x4 x[kAhead];
+            uint16_t sc[kAhead][kScales > 0 ? kScales : 1];
+            #pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + u * together + mine;
+                src[u] = of_lane(from, i & 63) + head * a.p.page.d;
+                dst[u] = of_lane(to, i & 63);
+                dst[u] = busy && i < last && dst[u] >= 0 ? dst[u] + head * a.p.page.d : -1;
             }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // (a row of this load may be where another goes)
-        #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (dst[u] >= 0) {
-                *reinterpret_cast<u32x4*>(pool + dst[u] * row_bytes(KIND, D) + 16 * piece) = x[u];
-                if constexpr (kScales > 0)
-                    if (piece == 0)
-                        for (int z = 0; z < kScales; ++z) scales[dst[u] * kScales + z] = sc[u][z];
-            }
+            #pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (dst[u] >= 0) {
+                    x[u] = *reinterpret_cast<const u32x4*>(pool + src[u] * row_bytes(KIND, D) + 16 * piece);
+                    if constexpr (kScales > 0)
+                        if (piece == 0)
+                            for (int z = 0; z < kScales; ++z) sc[u][z] = scales[src[u] * kScales + z];
+                }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // (a row of this load may be where another goes)
+            #pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (dst[u] >= 0) {
+                    *reinterpret_cast<u32x4*>(pool + dst[u] * row_bytes(KIND, D) + 16 * piece) = x[u];
+                    if constexpr (kScales > 0)
+                        if (piece == 0)
+                            for (int z = 0; z < kScales; ++z) scales[dst[u] * kScales + z] = sc[u][z];
+                }
+        }
     }
 }
 
