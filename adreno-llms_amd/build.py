@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmi_linear.so")
 SOURCES = ["runtime.hip", "gemv.hip", "gemm.hip", "argmax.hip", "decode.hip", "attention.hip", "kv_cache.hip",
-           "paged_attention.hip", "paged_tree.hip", "kv_move.hip", "rope.hip", "beam.hip", "probe.hip", "quantize.cpp", "bundle.cpp"]
+           "paged_attention.hip", "paged_tree.hip", "paged_tree_many.hip", "kv_move.hip", "rope.hip", "beam.hip", "probe.hip", "quantize.cpp", "bundle.cpp"]
 
 # -ffp-contract=off: the kernels spell every fused multiply-add as fmaf(); nothing else
 # may be fused, or results stop being bit-identical to the reference evaluation order.
@@ -26,7 +26,7 @@ DEVICE = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-pa
 
 # (attention.hip takes every result of a matrix product through the vector units at once: with the
 #  accumulators in the general registers a key tile of its main loop loses 116 register moves)
-PER_SOURCE = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("attention.hip", "paged_attention.hip", "paged_tree.hip")}
+PER_SOURCE = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("attention.hip", "paged_attention.hip", "paged_tree.hip", "paged_tree_many.hip")}
 
 
 def build(verbose=True, extra=()):

@@ -27,7 +27,7 @@ __device__ __forceinline__ int64_t row_number(const PagedArgs& a, int page, int 
            static_cast<uint32_t>(head * a.page.d + slot);
 }
 
-// paged_kernels.h: of mi_attention, and (TreeArgs) of mi_attention_tree
+// Of mi_attention, and (TreeArgs) of mi_attention_tree.
 struct AttentionArgs {
     PagedArgs p;
     const uint16_t* q;
@@ -43,6 +43,8 @@ struct TreeArgs : AttentionArgs {
     int words;
 };
 bool launch_paged_attention(hipStream_t s, const AttentionArgs& a, const StreamRoom& room);     // paged_attention.hip
+struct PagedLaunch;
 bool launch_paged_tree(hipStream_t s, const TreeArgs& a, const StreamRoom& room);               // paged_tree.hip
+bool launch_paged_tree_many(hipStream_t s, const TreeArgs& a, float* sums, uint32_t* counters, const PagedLaunch& l);      // paged_tree_many.hip
 
 }  // namespace mi

@@ -63,6 +63,7 @@ struct Room {                 // of the stream's workspace: for sums, and counte
 struct PagedLaunch {
     int wavefronts = 0;       // of 32 rows in a block of the kernel for many rows, 0: the kernel for few
     int slices = 1;           // of keys in such a block
+    int sets = 1;             // of 16 rows, of a wavefront of the kernel for trees
     Plan plan;
     int64_t blocks = 0;
     int threads = 0;
@@ -171,6 +172,38 @@ constexpr PagedLaunches attention_launches(const AttentionSize& a, const Room& r
         add(step_launch(a, room, cus, kFew));
     }
     return r;
+}
+
+// Which kernel serves a call of mi_attention_tree, always one for the whole batch: the one for few rows with 16 rows of a tree (its drafts times
+// the heads of a group) per wavefront or with 32 (paged_tree.hip), or the one for many rows in blocks of 128 (paged_tree_many.hip).  The
+// first reads and converts the keys again for every 16 or 32 rows, the last has a chain of 1.3 us (width 128: 2.6) per tile of 64 keys.
+// us, 16 rows / 32 / 128, W: tiles of 16 rows by 32 keys per compute unit, by the host's bounds of rows and lengths:
+//   width 64: 1 tree of 112 rows at 916 (W 2) 7.0 / 8.7 / 12.7; 8 of 28 at 8000 (31) 9.8 / 11.8 / 20.8; 1 of 448 at 4096 (28) 12.8 / 11.5 / 21;
+//     8 of 40 of 12 heads of their own at 3000 (107) 18.1 / 20.3 / 21.9; 13 of 300 in a window of 1024, Q4 (174) 23.6 / 19.9 / 24.5;
+//     8 of 224 at 8192 (225) 22.4 / 18.1 / 25.2; 32 of 168 at 4096 (355) int8 24.9 / 22.7 / 25.1, fp16 33.7 / 25.6 / 25.3;
+//     32 of 280 at 3000, Q4 (427) 26.9 / 21.8 / 24.7; 8 of 448 at 8192 (451) 33.5 / 25.9 / 26.1; 32 of 448 at 2000 (451) 35.5 / 26.6 / 22.9.
+//   width 128: 1 of 64 at 16000 (62) 24.6 / 25.7 / 45; 16 of 48 at 4000 (189) 32 / 38 / 37.6; 1 of 256 at 16000 (251) 75 / 51 / 78; 8 of 64 at
+//     16000 (500) 68 / 70 / 56; 32 of 256 at 2000 (1032) 106 / 93 / 87; 8 of 256 at 16384 (2064) fp16 265 / 194 / 116, int8 187 / 167 / 110.
+// Four sets of 16 rows to a wavefront spill registers and took 31 us for the 22.7 above.  At least 4 / 8 / 16 tiles to a block (4 wavefronts):
+// 112 rows at 916 (2) 6.8 / 7.6 / 8.8; 8 of 28 at 8000 (31) 15 / - / 9.8; 448 at 4096 (28) 14.5 / 11.5 / 11.5; 8 of 40 of 12 heads (107) 20.1 / - / 17.9.
+constexpr int kTreeFew = 64, kTreeTiny = 8, kTreeLittle = 16, kTreeMuch = 440;
+constexpr PagedLaunch tree_launch(const AttentionSize& a, const Room& room, int64_t cus) {
+    const int nrep = a.n_heads / a.n_kv_heads;
+    const int64_t rows = static_cast<int64_t>(a.max_tokens) * nrep;
+    int64_t keys = a.cap;
+    if (a.window > 0) {
+        const int64_t seen = static_cast<int64_t>(a.window) + a.sinks + a.max_tokens;
+        if (seen < keys) keys = seen;
+    }
+    const int64_t work = sets_at_most(a.n_tokens, a.n_seqs, nrep, kRows, 0, 0x7fffffff) * a.n_kv_heads * (keys / kKeys + 1);
+    if (work > kTreeMuch * cus && rows > kRows) return slices_launch(a, room, 4, 1, 0, 2 * cus);
+    const int sets = rows > kTreeFew && work > kTreeLittle * cus ? 2 : 1;
+    const int64_t want = a.head_dim == 64 ? (sets == 1 ? 4 : 2) * cus : (sets == 1 ? 2 : 1) * cus;
+    PagedLaunch l = make_launch(a, kRows * sets, 0, 0x7fffffff, want, room, sets * slot_floats(a.head_dim), 1);
+    l.plan.least = work > kTreeTiny * cus ? 4 * kWaves : kWaves;
+    l.sets = sets;
+    l.threads = 64 * kWaves;
+    return l;
 }
 
 // The blocks of a launch that has more threads than a grid counts; 0: none has.

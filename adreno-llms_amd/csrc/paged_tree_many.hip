@@ -1,0 +1,15 @@
+// Attention of trees of many rows over a cache in pages (mi_attention_tree): the kernel for many rows, in a file of its own so that
+// both compile at the same time.
+#include "paged_chunk.h"
+
+namespace mi {
+
+bool launch_paged_tree_many(hipStream_t s, const TreeArgs& a, float* sums, uint32_t* counters, const PagedLaunch& l) {
+    const PartRoom room = {sums, counters};
+    const bool wide = a.head_dim == 128;
+    return a.kind == MI_KV_F16    ? wide ? launch_chunk<MI_KV_F16, 128, 4, 1>(s, a, room, l) : launch_chunk<MI_KV_F16, 64, 4, 1>(s, a, room, l)
+           : a.kind == MI_KV_INT8 ? wide ? launch_chunk<MI_KV_INT8, 128, 4, 1>(s, a, room, l) : launch_chunk<MI_KV_INT8, 64, 4, 1>(s, a, room, l)
+                                  : wide ? launch_chunk<MI_KV_Q4, 128, 4, 1>(s, a, room, l) : launch_chunk<MI_KV_Q4, 64, 4, 1>(s, a, room, l);
+}
+
+}  // namespace mi
