@@ -40,6 +40,20 @@ constexpr int share_of(float all, const Plan& plan) {
     return share < plan.least ? plan.least : share;
 }
 
+// Items of a sequence where a block takes `share` tiles; and the least share, down to half of `share`, with which all sequences' items
+// (items(share), fewer the greater it is) are no more than `blocks`: `share` itself is known to fit.
+constexpr int items_of(const Cost& c, int share) { return c.sets ? c.sets * ((c.tiles - 1) / share + 1) : 0; }
+template <class Items>
+constexpr int even_share(int share, int blocks, const Items& items) {
+    int low = share / 2;                           // (not known to)
+    while (share - low > 1) {
+        const int mid = low + (share - low) / 2;
+        if (items(mid) <= blocks) share = mid;
+        else low = mid;
+    }
+    return share;
+}
+
 // Sets of rows_per_set rows that a launch over sequences of `from` to `to` rows has at most, whatever the lengths: every set full but
 // one of each sequence, of which there are no more than tokens and than times that `from` goes into all rows; and none longer than `to`.
 constexpr int64_t sets_at_most(int64_t n_tokens, int64_t n_seqs, int nrep, int rows_per_set, int from, int to) {

@@ -171,17 +171,11 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
             total += static_cast<float>(more.sets) * static_cast<float>(more.tiles);
         }
         it.share = uniform(share_of(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_to_last(total)), 63)), plan));
-        if (EVEN && a.p.n_seqs <= 64 && it.share >= 16) {
-            const float fit = static_cast<float>(gridDim.x / a.p.n_kv_heads);
-            int low = it.share / 2;                                  // (not known to fit)
-            #pragma unroll 1
-            while (it.share - low > 1) {
-                const int mid = (low + it.share) / 2;
-                const float items = c.sets ? static_cast<float>(c.sets * ((c.tiles - 1) / mid + 1)) : 0.0f;
-                if (__int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_to_last(items)), 63)) <= fit) it.share = mid;
-                else low = mid;
-            }
-            it.share = uniform(it.share);
+        if (EVEN && plan.target > 0 && a.p.n_seqs <= 64 && it.share >= 16) {
+            it.share = uniform(even_share(it.share, static_cast<int>(gridDim.x) / a.p.n_kv_heads, [&](int share) {
+                const float items = static_cast<float>(items_of(c, share));
+                return static_cast<int>(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_to_last(items)), 63)));
+            }));
         }
     }
     int before = 0;

@@ -19,10 +19,13 @@ def queue():
     return mil.Queue()
 
 
-@pytest.fixture(autouse=True, params=[0, 2 ** 20], ids=["tight", "wide"])
+COLUMNS = [0, 2 ** 14, 2 ** 20]
+
+
+@pytest.fixture(autouse=True, params=COLUMNS, ids=["tight", "middle", "wide"])
 def columns(request, monkeypatch):
-    """Small batches run on the kernel for few rows; under a page table for a million positions every sequence of more than 32 rows
-    runs on the one for many."""
+    """Small batches run on the kernel for few rows, 16 to a wavefront; under a page table for so many positions 32 to a wavefront, and
+    under one for a million on the kernel for many rows."""
     monkeypatch.setattr(Cache, "columns", request.param)
     return request.param
 
@@ -36,6 +39,8 @@ CASES = [
     dict(heads=15, kv_heads=5, D=64, page=100, lengths=[1500, 199, 101], new=[100, 99, 3], gap=3),
     dict(heads=8, kv_heads=1, D=128, page=32, lengths=[460, 333], new=[130, 129]),
     dict(heads=4, kv_heads=1, D=64, page=2048, lengths=[5000], new=[65], spare=0),
+    dict(heads=16, kv_heads=2, D=128, page=100, lengths=[300, 77], new=[30, 20]),
+    dict(heads=14, kv_heads=2, D=64, page=36, lengths=[90, 20], new=[12, 20]),
 ]
 
 
