@@ -208,3 +208,98 @@ def test_reorder_many_layers_and_bad_pages(queue):
                 for b in (1, 2, 3):
                     what[name][free[b], :, :8] = what[name][c.table[0, 2], :, :8]
         same(x.read_pools(), both)
+
+
+def test_pools_beyond_4_gib(queue):
+    """Pages at offsets that 32 bits do not hold: drafts attended, kept, and their sequence copied, out there."""
+    from tree_lib import TreeCache
+
+    page, kv, D, n_pages = 64, 8, 128, 36000
+    small = TreeCache(mil.KV_F16, 16, kv, D, page, [300, 70], [20, 30], seed=24)
+    size = kv * page * D * 2
+    assert n_pages * size > 2 ** 32
+    far = np.full_like(small.table, -1)
+    used = [(b, i) for b in range(2) for i in range(small.max_pages) if small.table[b, i] >= 0]
+    places = [n_pages - 1, 16384, 16383, 1, 35001, 32769, 20000][:len(used)]
+    pools = [mil.Buffer(n_pages * size) for _ in "kv"]
+    for (b, i), to in zip(used, places):
+        far[b, i] = to
+        for pool, name in zip(pools, "kv"):
+            host = np.ascontiguousarray(small.pool[name][small.table[b, i]])
+            assert mil.lib().mi_memcpy_h2d(pool.ptr + to * size, host.ctypes.data, size, None)
+    small.upload()
+    small.dev_table.write(far)
+    small.cache = mil.KVCache(mil.KV_F16, n_pages, page, kv, D, *pools)
+    small.check(small.attend(queue))
+
+    def rows(b, table, p):
+        """Keys and values at position p."""
+        got = []
+        for pool in pools:
+            host = np.empty((kv, page, D), np.uint16)
+            assert mil.lib().mi_memcpy_d2h(host.ctypes.data, pool.ptr + int(table[b, p // page]) * size, size, None)
+            got.append(host[:, p % page])
+        return np.array(got)
+
+    caches = mil.KVCaches([small.cache])
+    keep = np.full(50, -1, np.int32)
+    keep[:3], keep[20:22] = [1, 5, 19], [0, 29]
+    held = [mil.Buffer.from_host(x) for x in (keep, np.array([3, 2], np.int32))]
+    assert mil.kv_keep(queue, caches, small.batch, *held)
+    queue.finish()
+    for b, before, path in ((0, 280, [1, 5, 19]), (1, 40, [0, 29])):
+        for i, j in enumerate(path):
+            want = np.array([small.k[b][before + j], small.v[b][before + j]]).view(np.uint16)
+            assert (rows(b, far, before + i) == want).all()
+    lengths, source, fresh = np.array([283, 42], np.int32), np.array([1, 0], np.int32), np.array([35999 - 7, 33333], np.int32)
+    held = [mil.Buffer.from_host(x) for x in (lengths, far, source, fresh, np.zeros(2, np.int32), np.zeros_like(far))]
+    assert mil.kv_reorder(queue, caches, mil.ReorderCall(2, small.max_pages, *held))
+    queue.finish()
+    table = held[5].read(np.int32, far.shape)
+    assert table[0, 0] == fresh[0] and table[1].tolist() == [*far[0, :4], fresh[1]]
+    for b, f, p in ((0, 1, 0), (0, 1, 41), (1, 0, 256), (1, 0, 282)):
+        assert (rows(b, table, p) == rows(f, far, p)).all()
+
+
+def test_captured(queue):
+    """Graphs that follow paths, lengths and sources in device memory."""
+    c = Cache(mil.KV_INT8, 4, 4, 64, 16, [40, 33, 50], [20, 9, 30], seed=7, spare=6).upload()
+    free = [p for p in range(c.n_pages) if p not in set(c.table.ravel().tolist())][:3]
+    n = len(c.lengths)
+    buf = lambda x: mil.Buffer.from_host(np.array(x, np.int32))  # noqa: E731
+    keep, kept, new_len = buf([0] * c.rows), buf([0] * n), buf([0] * n)
+    source, fresh, after, table = buf(list(range(n))), buf(free), buf([0] * n), buf(c.table)
+    caches = mil.KVCaches([c.cache])
+    call = mil.ReorderCall(n, c.max_pages, new_len, c.dev_table, source, fresh, after, table)
+    assert mil.lib().mi_graph_begin(queue.handle)
+    assert mil.kv_keep(queue, caches, c.batch, keep, kept, new_len) and mil.kv_reorder(queue, caches, call)
+    graph = mil.lib().mi_graph_end(queue.handle)
+    assert graph
+    for turn in range(3):
+        rng = np.random.default_rng(turn)
+        paths = [np.sort(rng.choice(m, rng.integers(1, m), replace=False)) for m in c.new]
+        flat = np.full(c.rows, -1, np.int32)
+        for s, p in zip(c.start, paths):
+            flat[s:s + len(p)] = p
+        frm = rng.integers(0, n, n)
+        keep.write(flat)
+        kept.write(np.array([len(p) for p in paths], np.int32))
+        source.write(frm.astype(np.int32))
+        pools = c.read_pools()
+        lengths = [m - k + len(p) for m, k, p in zip(c.lengths, c.new, paths)]
+        for what in pools:
+            for name in "kv":
+                pool = what[name]
+                for b, p in enumerate(paths):
+                    at = c.lengths[b] - c.new[b]
+                    moved = pool[c.table[b][(at + p) // 16], :, (at + p) % 16].copy()
+                    to = at + np.arange(len(p))
+                    pool[c.table[b][to // 16], :, to % 16] = moved
+                for b, f in enumerate(frm):
+                    if f != b and lengths[f] % 16:
+                        pool[free[b], :, :lengths[f] % 16] = pool[c.table[f][lengths[f] // 16], :, :lengths[f] % 16]
+        assert mil.lib().mi_graph_launch(graph, queue.handle)
+        queue.finish()
+        same(c.read_pools(), pools)
+        assert after.read(np.int32, (n,)).tolist() == [lengths[f] for f in frm]
+    mil.lib().mi_graph_destroy(graph)
