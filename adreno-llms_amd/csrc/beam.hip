@@ -30,8 +30,7 @@ struct BeamArgs {
     int *out_token, *out_row;
     int64_t ld;
     int beams, vocab, n_out, tiles;
-    int first;                                     // group of the launch's first
-    int64_t rows;                                  // of the launch
+    int first, rows;                               // group of the launch's first; rows of the launch
 };
 
 // Sum of all lanes, in each of them.
@@ -108,11 +107,10 @@ __device__ __forceinline__ Scanned scan_tile(const uint16_t* row, int vocab, int
 }
 
 __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(const BeamArgs a, float2* __restrict__ sums, uint16_t* __restrict__ bins) {
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * kScanWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = item / a.tiles;
+    const int item = blockIdx.x * kScanWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = item / a.tiles;      // (few: they fit the workspace)
     if (row >= a.rows) return;
     const int lane = threadIdx.x & 63;
-    const Scanned s = scan_tile(a.logits + (static_cast<int64_t>(a.first) * a.beams + row) * a.ld, a.vocab, static_cast<int>(item - row * a.tiles));
+    const Scanned s = scan_tile(a.logits + (static_cast<int64_t>(a.first) * a.beams + row) * a.ld, a.vocab, item - row * a.tiles);
     bins[item * kBins + lane] = static_cast<uint16_t>(s.bin);
     if (lane == 0) sums[item] = float2{s.top, s.sum};
 }
@@ -589,7 +587,7 @@ extern "C" int mi_beam_select(void* stream, const mi_beam_call* call) {
     for (int64_t first = 0; first < c.n_groups; first += fit) {
         const int64_t n = c.n_groups - first < fit ? c.n_groups - first : fit, items = n * c.beams * a.tiles;
         a.first = static_cast<int>(first);
-        a.rows = n * c.beams;
+        a.rows = static_cast<int>(n * c.beams);
         auto* const bins = static_cast<uint16_t*>(workspace);
         auto* const sums = reinterpret_cast<float2*>(bins + items * kBins);
         hipLaunchKernelGGL(beam_scan_kernel, dim3(static_cast<unsigned>((items + kScanWaves - 1) / kScanWaves)), dim3(64 * kScanWaves), 0, s, a, sums,

@@ -24,7 +24,6 @@ struct RopeArgs {
     const int* position;
     int64_t ld_q, ld_k, ld_q_out, ld_k_out;
     int n_tokens, n_heads, heads, head_dim, pairs;     // heads: of q and k
-    int parts;                                         // wavefronts per row
     uint32_t axis[kMostPairs / 16];                    // of a pair, 2 bits each
 };
 
@@ -49,13 +48,13 @@ __device__ __forceinline__ uint16_t* to(const RopeArgs& a, int row, int head) {
     return head < a.n_heads ? a.q_out + row * a.ld_q_out + head * a.head_dim : a.k_out + row * a.ld_k_out + (head - a.n_heads) * a.head_dim;
 }
 
-// A wavefront has a row (or a part of its heads), a lane 16 elements of a head at a time: 8 pairs, or 16 of those behind them.  Where all
+// A wavefront has a row, a lane 16 elements of a head at a time: 8 pairs, or 16 of those behind them.  Where all
 // rows and halves are whole pieces of 16 bytes.
 template <bool SPLIT>
 __global__ __launch_bounds__(64 * kWaves) void rope_wide_kernel(const RopeArgs a) {
     __shared__ __attribute__((aligned(16))) float turn[kWaves][2 * kMostPairs];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int item = blockIdx.x * kWaves + wave, row = item / a.parts, part = item - row * a.parts;
+    const int row = blockIdx.x * kWaves + wave;
     if (row >= a.n_tokens) return;
     const int each = a.head_dim / 16, turning = a.pairs / 8, n = a.heads * each;
     struct Piece {
@@ -98,15 +97,14 @@ __global__ __launch_bounds__(64 * kWaves) void rope_wide_kernel(const RopeArgs a
         *reinterpret_cast<half8*>(p.dst + p.at_y) = p.y;
     };
     // (the first two pieces are on their way while the angles are worked out)
-    const int step = 64 * a.parts, z0 = part * 64 + lane;
     Piece now{}, next{};
-    if (z0 < n) now = load(z0);
-    if (z0 + step < n) next = load(z0 + step);
+    if (lane < n) now = load(lane);
+    if (lane + 64 < n) next = load(lane + 64);
     angles(a, row, lane, turn[wave]);
     __builtin_amdgcn_wave_barrier();
-    for (int z = z0; z < n; z += step) {
+    for (int z = lane; z < n; z += 64) {
         Piece after{};
-        if (z + 2 * step < n) after = load(z + 2 * step);
+        if (z + 128 < n) after = load(z + 128);
         finish(now);
         now = next;
         next = after;
@@ -118,12 +116,12 @@ template <bool SPLIT>
 __global__ __launch_bounds__(64 * kWaves) void rope_kernel(const RopeArgs a) {
     __shared__ float turn[kWaves][2 * kMostPairs];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int item = blockIdx.x * kWaves + wave, row = item / a.parts, part = item - row * a.parts;
+    const int row = blockIdx.x * kWaves + wave;
     if (row >= a.n_tokens) return;
     angles(a, row, lane, turn[wave]);
     __builtin_amdgcn_wave_barrier();
     const int rest = a.head_dim - 2 * a.pairs, each = a.pairs + rest, n = a.heads * each;
-    for (int z = part * 64 + lane; z < n; z += 64 * a.parts) {
+    for (int z = lane; z < n; z += 64) {
         const int head = z / each, i = z - head * each;
         const uint16_t* const src = from(a, row, head);
         uint16_t* const dst = to(a, row, head);
@@ -197,8 +195,7 @@ extern "C" int mi_rope(void* stream, const mi_rope_call* call) {
     a.n_heads = c.n_heads;
     a.heads = static_cast<int>(heads);
     a.head_dim = c.head_dim;
-    a.parts = 1;
-    const int64_t blocks = (static_cast<int64_t>(a.n_tokens) * a.parts + kWaves - 1) / kWaves;
+    const int64_t blocks = (static_cast<int64_t>(a.n_tokens) + kWaves - 1) / kWaves;
     if (blocks > 0x7fffffff / (64 * kWaves)) {
         MI_ERROR_FMT("mi_rope: %d rows are more than a launch counts", c.n_tokens);
         return 0;

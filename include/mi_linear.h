@@ -147,7 +147,8 @@ int mi_linear_argmax_static(void* stream, int N, int K, const void* x, const voi
  * of logits (fp16 [n_groups * beams], ld elements apart, `vocab` of them) and score (fp32, the sum of log probabilities so far) are group
  * g's.  Its n_out best continuations are left, best first, in out_score, out_token and out_row [n_groups][n_out]: token t of row r counts
  *   score[r] + logits[r][t] - log sum_u exp logits[r][u],
- * compared in 64 bits and left as fp32; among equals the lowest row, then the lowest token.  -infinity is a logit that is never chosen (a
+ * compared in 64 bits and left as fp32; among equals the lowest row, then the lowest token (scores up to 2^28 in size: beyond, the sums
+ * of one row's different logits are equal).  -infinity is a logit that is never chosen (a
  * token that a grammar forbids); a row whose score is not finite (a beam that is not there, the others of a first step), whose
  * logits are all -infinity, or that holds a NaN or +infinity is never chosen from.  Where fewer than n_out are left the others are
  * -infinity, -1, -1.  out_row is a number of all rows, as mi_kv_reorder takes it.  With n_out = 2 * beams a host has enough whichever
