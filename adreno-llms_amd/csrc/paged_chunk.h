@@ -26,6 +26,11 @@ namespace {
 constexpr int chunk_lds(int D) { return 2 * 2 * kChunkKeys * 2 * D; }          // of a slice's tiles
 constexpr int chunk_lds_all(int D, int KS) { return KS * (chunk_lds(D) + 2 * kChunkKeys); }
 constexpr int meet_floats(int D, int RW) { return RW * 64 * (D / 2 + 3); }         // of a slice's sums
+__device__ const __attribute__((aligned(16))) uint32_t kNothing[4] = {0, 0, 0, 0};
+// 16 bytes from each lane's place in memory to LDS, the lanes' side by side from `to` on (which is the wavefront's).
+__device__ __forceinline__ void lds_fill(const uint8_t* from, uint8_t* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint8_t*)from, (__attribute__((address_space(3))) uint8_t*)to, 16, 0, 0);
+}
 __device__ __forceinline__ constexpr int twist(int row) { return (row & 3) * 2 + (row >> 2 & 1); }
 
 // Dear: a row takes its keys one to a lane and its values one after the other.  A prompt of 2048 rows of 14 heads over 2 with one NaN among
@@ -165,6 +170,26 @@ __global__ __launch_bounds__(64 * RW * KS, is_tree<Args> && D == 64 ? 3 : 2) voi
             }
             // what is not in the cache becomes zeros
             if (bad || j0 + p * kPer + my_row >= tiles.end) raw.none |= 1u << p;
+        }
+    };
+    // A tree's tile in fp16 goes from its pages to LDS by itself, a row's piece p ^ twist(row) to the place p (what is not in the cache from a
+    // piece of zeros).
+    auto fill = [&](int v, const Pages& g, int buf) {
+        const int j0 = tile_at(tiles, v) * kChunkKeys;
+        uint8_t* const kt = own_lds + buf * (chunk_lds(D) / 2) + wave * 1024;
+        #pragma unroll
+        for (int p = 0; p < kLoads; ++p) {
+            const int j = key_of(j0, p), number = g.number[p], row = p * kPer + my_row;
+            const bool bad = static_cast<uint32_t>(number) >= static_cast<uint32_t>(a.p.n_pages), none = bad || j0 + row >= tiles.end;
+            int slot = j - divide(j, a.p.page) * a.p.page.d;
+            if constexpr (PAGES16) slot &= ~15;
+            const int64_t at = row_number(a.p, bad ? 0 : number, kvh, slot);
+            const uint32_t off = (PAGES16 ? my_row & 15 : 0) * kRow + (my_piece ^ twist(my_row)) * kPiece;
+            const uint8_t *kb = a.p.k + at * kRow + off, *vb = a.p.v + at * kRow + off;
+            if (none) kb = vb = reinterpret_cast<const uint8_t*>(kNothing);
+            lds_fill(kb, kt + p * kPer * (2 * D));
+            lds_fill(vb, kt + p * kPer * (2 * D) + chunk_lds(D) / 4);
+            if (my_piece == 0) gone[buf * kChunkKeys + row] = none;
         }
     };
     uint32_t exponent = 0x64006400u;
@@ -348,18 +373,30 @@ __global__ __launch_bounds__(64 * RW * KS, is_tree<Args> && D == 64 ? 3 : 2) voi
     Pages pages;
     const int mine = first + slice;
     auto clamp = [&](int v) { return v < last ? v : last - 1; };
+    constexpr bool kStraight = kTree && KIND == MI_KV_F16 && KS == 1;
     if (first < last) {
         pages = look_up(mine);
-        fetch(clamp(mine), pages);
+        if constexpr (kStraight) fill(mine, pages, 0);
+        else fetch(clamp(mine), pages);
         pages = look_up(mine + KS);
     }
     for (int v = mine, buf = 0; v - slice < last; v += KS, buf ^= 1) {
-        stash(buf);
-        if (v - slice + KS < last) {
-            fetch(clamp(v + KS), pages);
-            pages = look_up(v + 2 * KS);
+        if constexpr (kStraight) {
+            // (this tile is there, and the one before it done with, for all wavefronts)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (v + 1 < last) {
+                fill(v + 1, pages, buf ^ 1);
+                pages = look_up(v + 2);
+            }
+        } else {
+            stash(buf);
+            if (v - slice + KS < last) {
+                fetch(clamp(v + KS), pages);
+                pages = look_up(v + 2 * KS);
+            }
+            __syncthreads();
         }
-        __syncthreads();
         if (v < last) {
             const int j0 = tile_at(tiles, v) * kChunkKeys;
             const int w_first = a.window > 0 && p_lo >= a.window ? p_lo - a.window + 1 : 0;    // of the window of the wavefront's first query
