@@ -1,4 +1,4 @@
-// Which kernels serve a call of mi_attention (paged_attention.hip), with how many blocks, and how the keys of sequences are shared
+// Which kernels serve a call of mi_attention (paged_attention.hip) or mi_attention_tree (paged_tree.hip), with how many blocks, and how the keys of sequences are shared
 // out to them: everything that follows from the numbers the host has, and from a sequence's lengths.  Plain C++ (constexpr makes
 // device code as well).
 #pragma once

@@ -1,4 +1,4 @@
-// What the kernels over a paged cache (kv_cache.hip, paged_attention.hip) take from the numbers that a call leaves in device
+// What the kernels over a paged cache (kv_cache.hip, kv_move.hip, paged_attention.hip, paged_tree.hip) take from the numbers that a call leaves in device
 // memory: where a row lies, what a query sees, which tiles of keys a group of queries has, and how tiles are shared out to
 // blocks.  Every such number is checked here, so that no value of it leads out of the caller's arrays.  Plain C++
 // (constexpr makes device code as well).

@@ -13,7 +13,7 @@ constexpr int kSliceCounters = 16384;
 inline uint32_t* slice_counters(void* workspace) {
     return reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + kWorkspaceBytes);
 }
-// An allocation of its own: room for the sums of attention's rows whose keys several blocks share (paged_attention.hip).
+// An allocation of its own: room for the sums of attention's rows whose keys several blocks share (paged_attention.hip, paged_tree.hip).
 constexpr size_t kPartialBytes = 32u << 20;
 
 struct StreamRoom {
