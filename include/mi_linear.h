@@ -153,7 +153,7 @@ int mi_linear_argmax_static(void* stream, int N, int K, const void* x, const voi
  * logits are all -infinity, or that holds a NaN or +infinity is never chosen from.  Where fewer than n_out are left the others are
  * -infinity, -1, -1.  out_row is a number of all rows, as mi_kv_reorder takes it.  With n_out = 2 * beams a host has enough whichever
  * of them end.  The reference decodes greedily or samples; it has no beams.
- * beams and n_out 1 to 64, vocab up to MI_BEAM_MAX_VOCAB.  Two launches on a stream of mi_stream_create or the null stream, whose
+ * The outputs overlap nothing.  beams and n_out 1 to 64, vocab up to MI_BEAM_MAX_VOCAB.  Two launches on a stream of mi_stream_create or the null stream, whose
  * workspace holds the rows' sums and maxima in between; on any other stream one launch, slower.  Nothing is allocated or waited for. */
 #define MI_BEAM_MAX_VOCAB (1 << 21)
 typedef struct mi_beam_call {

@@ -183,3 +183,45 @@ def test_captured(queue):
         got = [o.read(t, (groups, n_out)) for o, t in zip(outs, (np.float32, np.int32, np.int32))]
         check(got, expect(logits, score, groups, beams, n_out))
     mil.lib().mi_graph_destroy(graph)
+
+
+def test_streams_at_once(queue):
+    """Two streams, each with a workspace of its own."""
+    rng = np.random.default_rng(11)
+    queues, held, calls, outs = [queue, mil.Queue()], [], [], []
+    for i in range(2):
+        logits, score = make(rng, 8, 30000)
+        held.append((logits, score, mil.Buffer.from_host(logits), mil.Buffer.from_host(score)))
+        outs.append([mil.Buffer.from_host(np.zeros((2, 8), np.int32)) for _ in range(3)])
+        calls.append(mil.BeamCall(2, 4, 30000, 8, *held[i][2:], *outs[i]))
+    for _ in range(30):
+        for q, call in zip(queues, calls):
+            assert mil.beam_select(q, call)
+    for q, (logits, score, _, _), out in zip(queues, held, outs):
+        q.finish()
+        check([o.read(t, (2, 8)) for o, t in zip(out, (np.float32, np.int32, np.int32))], expect(logits, score, 2, 4, 8))
+
+
+@pytest.mark.parametrize("beams", [1, 2, 8, 9, 16, 17, 33, 64])
+@pytest.mark.parametrize("n_out", [1, 2, 16, 24, 25, 63, 64])
+def test_every_number_of_beams_and_outputs(queue, beams, n_out):
+    """Scores nearly alike, so that all rows offer; among them rows that tie in everything, and logits of few values."""
+    rng = np.random.default_rng(beams * 100 + n_out)
+    for levels in (0, 5, 400):
+        logits, score = make(rng, 2 * beams, 5000)
+        if levels:
+            logits = (np.rint(logits.astype(np.float32) * levels / 8) * 8 / levels).astype(np.float16)
+        score[:] = np.where(rng.random(2 * beams) < 0.5, -20, score / 100 - 20)
+        logits[beams:][::3] = logits[beams]
+        score[beams:][::3] = score[beams]
+        check(select(queue, logits, score, 2, beams, 5000, n_out), expect(logits, score, 2, beams, n_out))
+
+
+@pytest.mark.parametrize("score", [1e6, -3e7, 2.0 ** 28])
+def test_scores_far_from_zero(queue, score):
+    """The order is that of the 64-bit sums, which fp32's steps at the scores do not show."""
+    rng = np.random.default_rng(12)
+    logits, _ = make(rng, 4, 3000)
+    scores = np.full(4, score, np.float32)
+    got, want = select(queue, logits, scores, 1, 4, 3000, 12), expect(logits, scores, 1, 4, 12)
+    assert (got[1] == want[1]).all() and (got[2] == want[2]).all() and (got[0] == want[0].astype(np.float32)).all()

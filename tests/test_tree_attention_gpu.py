@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from helpers import mil
-from paged_lib import Cache
+from paged_lib import Cache, quantise, values
 from tree_lib import TreeCache, ancestors
 
 pytestmark = pytest.mark.gpu
@@ -164,3 +164,98 @@ def test_a_stream_without_a_workspace(queue):
     assert hip.hipStreamSynchronize(foreign) == 0
     c.check(out.read(np.float16, (c.rows, c.heads, c.D)))
     assert hip.hipStreamDestroy(foreign) == 0
+
+
+class Odd(TreeCache):
+    """Sequences whose lengths or pages on the device are not those that the cache was made with."""
+
+    def bend(self, lengths=None, table=None):
+        if lengths is not None:
+            self.bent = list(lengths)
+            self.dev_len.write(np.array(lengths, np.int32))
+        if table is not None:
+            self.bent_table = table
+            self.dev_table.write(table)
+        return self
+
+    def visible(self, b, window, sinks):
+        n, m = self.new[b], self.lengths[b]
+        end, base = self.bent[b], self.bent[b] - n
+        seen = np.zeros((n, m), bool)
+        for p in range(min(m, max(end, 0))):
+            page = self.bent_table[b, p // self.page]
+            if not 0 <= page < self.n_pages:
+                continue
+            if p < base:
+                place = np.clip(self.position[self.start[b]:self.start[b] + n], base, end - 1)
+                seen[:, p] = (p > place - window) | (p < sinks) if window > 0 else True
+            else:
+                seen[:, p] = self.masks[b][:, p - base]
+        return seen
+
+
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("kind", [mil.KV_F16, mil.KV_Q4])
+def test_lengths_and_pages_that_do_not_fit(queue, kind, window):
+    """Fewer positions than drafts (the first ones have no place), none, less than none; pages that are not in the pool."""
+    c = Odd(kind, 14, 2, 64, 16, [60, 40, 33, 50, 90], [16, 20, 20, 9, 30], seed=11).upload()
+    table = c.table.copy()
+    table[0, 1], table[4, 2], table[4, 5] = -1, c.n_pages, 2 ** 31 - 1
+    c.bend([60, 13, 0, -5, 90], table)
+    got = c.attend(queue, window=window, sinks=3)
+    c.check(got, window, 3)
+    assert (got[36:65] == 0).all()
+
+
+def test_many_sequences_and_wrong_hints(queue):
+    """More than the 64 that are planned at a time, of all sizes; max_tokens says how many there are at most, or does not."""
+    rng = np.random.default_rng(12)
+    new = [int(x) for x in rng.integers(0, 9, 150)]
+    new[77] = 60
+    c = TreeCache(mil.KV_F16, 9, 3, 64, 16, [n + int(rng.integers(0, 60)) for n in new], new, seed=12, pad=5).upload()
+    want = c.expect()
+    for hint in (60, 0, 1, 7, 5000):
+        c.batch.max_tokens = hint
+        got = c.attend(queue)[:sum(new)].astype(np.float64)
+        assert (np.abs(got - want[0]) <= want[1]).all(), hint
+
+
+def test_streams_at_once(queue):
+    """Two streams, each with a workspace of its own, and parts that meet in it."""
+    queues = [queue, mil.Queue()]
+    caches = [TreeCache(mil.KV_F16, 14, 2, 64, 16, [3000 + 77 * i], [40], seed=13 + i).upload() for i in range(2)]
+    calls = []
+    for c in caches:
+        out = mil.Buffer.from_host(np.zeros((c.rows, c.heads * c.D), np.uint16))
+        mask = mil.TreeMask(mil.Buffer.from_host(np.ascontiguousarray(c.seen)), c.words)
+        calls.append((mil.AttentionCall(c.cache, c.batch, c.heads, c.dev_qkv, out, ld_q=c.ld), mask, out))
+    for _ in range(20):
+        for q, (call, mask, _out) in zip(queues, calls):
+            assert mil.attention_tree(q, call, mask)
+    for q, c, (_call, _mask, out) in zip(queues, caches, calls):
+        q.finish()
+        c.check(out.read(np.float16, (c.rows, c.heads, c.D)))
+
+
+@pytest.mark.parametrize("scale", [1e-30, 300.0, 65504.0])
+@pytest.mark.parametrize("kind", [mil.KV_F16, mil.KV_INT8])
+def test_scales(queue, kind, scale):
+    """Weights all alike, and scores of thousands and millions, whose products are rounded before the base is taken off."""
+    c = TreeCache(kind, 14, 2, 64, 16, [200, 90], [40, 7], seed=14).upload()
+    got = c.attend(queue, scale=scale)
+    assert np.isfinite(got[:47]).all()
+    if scale < 1:
+        c.check(got, scale=scale)
+    else:                                                 # the greatest score has (nearly) all the weight
+        for b, (n, m) in enumerate(zip(c.new, c.lengths)):
+            k, v = (values(kind, *quantise(kind, x[b])).astype(np.float64) for x in (c.k, c.v))
+            seen = c.visible(b, 0, 0)
+            for r in range(n):
+                for h in range(c.heads):
+                    s = k[:, h // 7] @ c.qkv[c.start[b] + r, h * 64:(h + 1) * 64].astype(np.float64) * scale
+                    s[~seen[r]] = -np.inf
+                    order = np.argsort(-s)
+                    # a second score may take weight where it is within fp32's error of the sum (64 2^-24 of it) and 20 of the first
+                    if s[order[0]] - s[order[1]] > 20 + 2.0 ** -17 * np.abs(s[order[0]]):
+                        want = v[order[0], h // 7]
+                        assert (np.abs(got[c.start[b] + r, h] - want) <= 2.0 ** -9 * np.abs(want) + 2.0 ** -16).all()
