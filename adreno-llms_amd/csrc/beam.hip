@@ -345,6 +345,7 @@ __device__ __forceinline__ int pick(const uint16_t* row, int vocab, int tiles, c
 constexpr int kGroupWaves = 2 * kPickWaves, kGroupThreads = 64 * kGroupWaves;
 constexpr int kOffer = 64;                         // offers of a row at most
 constexpr int kIdBits = 21;                        // of the token
+constexpr int kSame = 8;
 struct Offer {
     double value;
     uint32_t id, pad;                              // row of the group and token
@@ -355,10 +356,11 @@ __device__ __forceinline__ uint32_t key_of(double value) {
     const uint32_t u = __float_as_uint(static_cast<float>(value));
     return u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
 }
-struct Choice {                                    // in LDS, the rows' offers behind it
+struct __attribute__((aligned(16))) Choice {       // in LDS, the rows' offers behind it
     uint32_t keys[kGroupThreads + 4];              // of all offers, one row's behind the other's
     uint16_t slots[kGroupThreads];
     int places[kGroupThreads], hits[kMostOut];
+    uint16_t same[kMostOut][kSame];                // offers that share a place
     double offsets[kMostBeams];
     int counts[kMostBeams];
     Offer offers[1];
@@ -441,25 +443,33 @@ __device__ __forceinline__ int merge_few(const BeamArgs& a, int64_t group, Choic
     if (tid < kMostOut) c.hits[tid] = 0;
     if (tid < 4) c.keys[all + tid] = 0;
     __syncthreads();
-    const int chunks = (all + 63) / 64, parts = chunks ? kGroupWaves / chunks : 1, chunk = wave % (chunks ? chunks : 1), part = wave / (chunks ? chunks : 1);
-    const int mine = chunk * 64 + lane;
-    if (part < parts && mine < all) {
+    const int chunks = (all + 63) / 64, shift = chunks > 1 ? 32 - __builtin_clz(chunks - 1) : 0;       // 2^shift times 64 offers are room for all
+    const int parts = kGroupWaves >> shift, part = wave >> shift, mine = (wave - (part << shift)) * 64 + lane;
+    if (mine < all) {
         const uint32_t key = c.keys[mine];
         int place = 0;
-        #pragma unroll 2
+        #pragma unroll 4
         for (int z = 4 * part; z < all; z += 4 * parts) {
+            const u32x4 other = *reinterpret_cast<const u32x4*>(&c.keys[z]);
             #pragma unroll
-            for (int e = 0; e < 4; ++e) place += c.keys[z + e] > key;
+            for (int e = 0; e < 4; ++e) place += other[e] > key;
         }
         if (place) atomicAdd(&c.places[mine], place);
     }
     __syncthreads();
     int place = tid < all ? c.places[tid] : a.n_out;
-    if (place < a.n_out) atomicAdd(&c.hits[place], 1);
+    if (place < a.n_out) {
+        const int nth = atomicAdd(&c.hits[place], 1);
+        if (nth < kSame) c.same[place][nth] = static_cast<uint16_t>(tid);
+    }
     __syncthreads();
     if (place < a.n_out) {
         const Offer o = c.offers[c.slots[tid]];
-        if (c.hits[place] > 1) {
+        const int hits = c.hits[place], shared = place;
+        if (hits > 1 && hits <= kSame) {           // (two tokens of a row have the same logit, most often)
+            #pragma unroll 1
+            for (int z = 0; z < hits; ++z) place += better(c.offers[c.slots[c.same[shared][z]]], o);
+        } else if (hits > 1) {
             const uint32_t key = c.keys[tid];
             #pragma unroll 1
             for (int z0 = 0; z0 < all; z0 += 4) {
