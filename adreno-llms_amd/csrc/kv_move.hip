@@ -174,7 +174,8 @@ __global__ __launch_bounds__(kCopyThreads) void kv_reorder_kernel(const ReorderA
 
 bool off(const void* p, uintptr_t align) { return !p || reinterpret_cast<uintptr_t>(p) % align; }
 
-// Checks the caches of a call, which are alike but for their pools, and its batch.
+// Checks the caches of a call, which are alike but for their pools, and its batch.  (A pool that is there twice would have its rows moved twice,
+// by two wavefronts at once.  Every pool is compared with all before it: half a microsecond for 32 caches.)
 bool layers_args(const char* who, const mi_kv_cache* caches, int n, const mi_kv_batch& batch, PagedArgs* out) {
     if (!caches || n < 1) {
         MI_ERROR_FMT("%s: no caches (caches=%p n_caches=%d)", who, static_cast<const void*>(caches), n);
@@ -185,6 +186,15 @@ bool layers_args(const char* who, const mi_kv_cache* caches, int n, const mi_kv_
         if (!paged_args(who, &c, &batch, out)) return false;
         if (c.kind != d.kind || c.n_pages != d.n_pages || c.page_size != d.page_size || c.n_kv_heads != d.n_kv_heads || c.head_dim != d.head_dim) {
             MI_ERROR_FMT("%s: cache %d differs from the first in more than its pools", who, i);
+            return false;
+        }
+    }
+    for (int i = 0; i < n; ++i) {
+        bool twice = caches[i].k == caches[i].v;
+        for (int j = 0; j < i; ++j)
+            twice |= (caches[j].k == caches[i].k) | (caches[j].k == caches[i].v) | (caches[j].v == caches[i].k) | (caches[j].v == caches[i].v);
+        if (twice) {
+            MI_ERROR_FMT("%s: a pool of cache %d is there twice", who, i);
             return false;
         }
     }
@@ -223,7 +233,7 @@ extern "C" int mi_kv_keep(void* stream, const mi_kv_cache* caches, int n_caches,
     KeepArgs a{};
     if (!layers_args("mi_kv_keep", caches, n_caches, *batch, &a.p)) return 0;
     if (a.p.n_seqs == 0) return 1;
-    if ((a.p.n_tokens > 0 && off(keep, 4)) || off(kept, 4) || (new_len && (off(new_len, 4) || new_len == kept || new_len == a.p.kv_len))) {
+    if ((a.p.n_tokens > 0 && off(keep, 4)) || off(kept, 4) || (new_len && (off(new_len, 4) || new_len == keep || new_len == kept || new_len == a.p.q_start || new_len == a.p.kv_len || new_len == a.p.pages))) {
         MI_ERROR_FMT("mi_kv_keep: bad argument (keep=%p kept=%p new_len=%p)", static_cast<const void*>(keep), static_cast<const void*>(kept),
                      static_cast<void*>(new_len));
         return 0;

@@ -140,7 +140,7 @@ int mi_attention_tree(void* stream, const mi_attention_call* call, const mi_tree
  * n_b earlier positions, the rows numbered keep[q_start[b] + i], i = 0 .. kept[b] - 1, ascending, each of 0 .. n_b - 1, become
  * positions before + i, in every cache of `caches`; what the other positions hold is left as it is.  new_len[b] = before + kept[b] (kept
  * taken as within 0 .. n_b; less than 0 counts as 0) unless new_len is null; it overlaps none of the arrays that are read.
- * caches: n_caches of them, the layers of a model say, which differ in their pools alone.  keep [n_tokens] (what lies behind a
+ * caches: n_caches of them, the layers of a model say, which differ in their pools alone; no pool is there twice.  keep [n_tokens] (what lies behind a
  * sequence's kept ones is not read), kept [n_seqs], new_len [n_seqs]: device memory, 4-byte aligned.  Rows move as they are stored.  A row
  * or a place that is not in the cache, or a number out of range, moves nothing.  Where numbers do not ascend it is not said
  * which rows end up where, but no other positions are touched.  No two sequences of a call share a page that holds a new row. */

@@ -154,3 +154,20 @@ def test_beam_null_and_nothing(capfd):
 def test_good_calls_go_on_to_the_device(capfd):
     assert not any((rope(), tree(), keep(), reorder(), beam()))
     assert "bad" not in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("pools,which", [
+    ([(4096, 8192), (16384, 32768), (4096, 65536)], 2), ([(4096, 8192), (8192, 16384)], 1), ([(4096, 4096)], 0),
+    ([(4096, 8192), (16384, 8192)], 1), ([(4096, 8192), (16384, 32768), (65536, 16384)], 2),
+])
+def test_a_pool_that_is_there_twice(capfd, pools, which):
+    """Its rows would be moved twice, by two wavefronts at once."""
+    caches = [dict(k=k, v=v) for k, v in pools]
+    assert not keep(caches) and not reorder(caches)
+    err = capfd.readouterr().err
+    assert err.count(f"a pool of cache {which} is there twice") == 2, err
+
+
+def test_lengths_do_not_replace_what_is_read(capfd):
+    assert not keep(new_len=256, keep=256) and not keep(new_len=BATCH["pages"]) and not keep(new_len=BATCH["q_start"])
+    assert capfd.readouterr().err.count("bad argument") == 3
