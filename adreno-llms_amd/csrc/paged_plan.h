@@ -54,6 +54,28 @@ constexpr int even_share(int share, int blocks, const Items& items) {
     return share;
 }
 
+// The sets of a sequence read the same keys.  Blocks go to the eight XCDs in turn, each with an L2 of its own: so that a part of the keys of a
+// key/value head (a pair) meets all its sets in one L2, they are eight blocks apart, one behind the other.  The sets and pairs of a sequence's blocks in
+// their order, block `in`; pairs behind the last whole eight lie side by side.
+// With the sets as far apart as a head has parts, key/value heads that do not go into eight spread them over all XCDs; and where one sequence is all there
+// is its sets read their keys at other times.  us for few rows (paged_tree.hip), that way / eight apart: 32 trees of 24, 15 heads over 5, behind 4096, fp16 38.7 /
+// 32.5; 8 of 16 behind 16384, 28 over 7, width 128 fp16 102 / 67, int8 61 / 50; 16 of 24 behind 4096, int8, 15 over 5 16.5 / 17.0 (the worst); one tree of 24
+// behind 16384, 12 over 6 25.6 / 18.0, 14 over 2 22.9 / 18.8, 32 over 8 22.0 / 19.5, width 128 47.2 / 47.5.  Else there is little in it: 16 of 24
+// behind 4096, int8, 14 over 2 15.0 / 16.0, 8 of 16 behind 16384 28.8 / 27.5.  For many rows (paged_tree_many.hip) nothing: 0.96 to 1.05.
+struct SetOfPair {
+    unsigned set, pair;
+};
+constexpr SetOfPair eight_apart(unsigned in, unsigned sets, unsigned pairs) {
+    const unsigned group = 8 * sets, whole = pairs / 8 * group;
+    if (in < whole) {
+        const unsigned at = in / group, within = in - at * group;
+        return {within / 8, at * 8 + within % 8};
+    }
+    const unsigned rest = pairs % 8, set = (in - whole) / rest;
+    return {set, pairs / 8 * 8 + (in - whole - set * rest)};
+}
+constexpr bool eight_apart_pays(int n_seqs, int n_kv_heads) { return n_seqs == 1 || 8 % n_kv_heads != 0; }
+
 // Sets of rows_per_set rows that a launch over sequences of `from` to `to` rows has at most, whatever the lengths: every set full but
 // one of each sequence, of which there are no more than tokens and than times that `from` goes into all rows; and none longer than `to`.
 constexpr int64_t sets_at_most(int64_t n_tokens, int64_t n_seqs, int nrep, int rows_per_set, int from, int to) {
@@ -196,7 +218,7 @@ constexpr PagedLaunches attention_launches(const AttentionSize& a, const Room& r
 //     8 of 40 of 12 heads of their own at 3000 (107) 18.1 / 20.3 / 21.9; 13 of 300 in a window of 1024, Q4 (174) 23.6 / 19.9 / 24.5;
 //     8 of 224 at 8192 (225) 22.4 / 18.1 / 25.2; 32 of 168 at 4096 (355) int8 24.9 / 22.7 / 25.1, fp16 33.7 / 25.6 / 25.3;
 //     32 of 280 at 3000, Q4 (427) 26.9 / 21.8 / 24.7; 8 of 448 at 8192 (451) 33.5 / 25.9 / 26.1; 32 of 448 at 2000 (451) 35.5 / 26.6 / 22.9.
-//   width 128: 1 of 64 at 16000 (62) 24.6 / 25.7 / 45; 16 of 48 at 4000 (189) 32 / 38 / 37.6; 1 of 256 at 16000 (251) 75 / 51 / 78; 8 of 64 at
+//   width 128: 1 of 64 at 16000 (62) 26.8 / 25.7 / 45; 16 of 48 at 4000 (189) 32 / 38 / 37.6; 1 of 256 at 16000 (251) 75 / 50 / 74; 8 of 64 at
 //     16000 (500) 68 / 70 / 56; 32 of 256 at 2000 (1032) 106 / 93 / 87; 8 of 256 at 16384 (2064) fp16 265 / 194 / 116, int8 187 / 167 / 110.
 // Four sets of 16 rows to a wavefront spill registers and took 31 us for the 22.7 above.  At least 4 / 8 / 16 tiles to a block (4 wavefronts):
 // 112 rows at 916 (2) 6.8 / 7.6 / 8.8; 8 of 28 at 8000 (31) 15 / - / 9.8; 448 at 4096 (28) 14.5 / 11.5 / 11.5; 8 of 40 of 12 heads (107) 20.1 / - / 17.9.

@@ -141,6 +141,7 @@ __device__ __forceinline__ uint32_t drafts_seen(const TreeArgs& a, const Span& s
 struct Item {
     int b = -1, set = 0, chunk = 0, share = 0, tiles = 0;
     Span s;
+    int kvh = 0, id = 0;      // its key/value head, and its number over all of them: the parts of a set are n_kv_heads apart
 };
 
 // Item `y` of the batch (of any one key/value head); b = -1: there is none.  A q_start that goes down somewhere has more rows than the
@@ -149,7 +150,8 @@ struct Item {
 //
 // EVEN: where a block's share is long, the least share is looked for with which the items still fit the launch's blocks: the first one leaves
 // a part of a share in the last part of each set, up to half of all (at 16 tiles and more: it takes about a microsecond).
-template <int ROWS, int KEYS, bool EVEN = false>
+// NEAR: which of a sequence's items a block has is as eight_apart says, where that pays.
+template <int ROWS, int KEYS, bool EVEN = false, bool NEAR = false>
 __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan, const int y) {
     const int lane = threadIdx.x & 63;
     bool down = false;
@@ -192,6 +194,20 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
             it.tiles = __builtin_amdgcn_readlane(c.tiles, l);
             const int n = __builtin_amdgcn_readlane(chunks, l), sets = __builtin_amdgcn_readlane(c.sets, l);
             const int own = y - (__builtin_amdgcn_readlane(upto, l) - sets * n);
+            if constexpr (NEAR) {
+                const unsigned heads = a.p.n_kv_heads;
+                it.id = blockIdx.x;
+                it.kvh = blockIdx.x - y * heads;
+                if (sets > 1 && eight_apart_pays(a.p.n_seqs, heads)) {
+                    const SetOfPair x = eight_apart(own * heads + it.kvh, sets, n * heads);
+                    it.set = x.set;
+                    it.chunk = x.pair / heads;
+                    it.kvh = x.pair - it.chunk * heads;
+                    it.id = (y - own + x.set * n + it.chunk) * heads + it.kvh;
+                    if (n > 1) it.share = (it.tiles - 1) / n + 1;
+                    return it;
+                }
+            }
             const int set = sets == 1 ? 0 : own / n;
             it.chunk = own - set * n;
             it.set = sets - 1 - set;                                 // (the longest first)

@@ -43,9 +43,9 @@ __global__ __launch_bounds__(64 * kWaves, tree_blocks(KIND, D, PAGES16, SETS)) v
     __shared__ uint32_t arrived;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % a.p.n_kv_heads, y = blockIdx.x / a.p.n_kv_heads;
-    const Item it = item_of<kRows * SETS, kKeys>(a, plan, y);
+    const Item it = item_of<kRows * SETS, kKeys, false, true>(a, plan, blockIdx.x / a.p.n_kv_heads);
     if (it.b < 0) return;
+    const int kvh = it.kvh;
     const int rows = it.s.n * plan.nrep, r0 = it.set * (kRows * SETS), r_end = r0 + kRows * SETS < rows ? r0 + kRows * SETS : rows;
     const int base_pos = it.s.pos, p_hi = it.s.pos + (it.s.n - 1);                // of the first draft, of the last
     const Tiles tiles = tiles_of(base_pos, p_hi, a.p.cap, a.window, a.sinks, kKeys);
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(64 * kWaves, tree_blocks(KIND, D, PAGES16, SETS)) v
         // The parts of a set meet in memory, at agent scope, which passes the XCDs' own L2s; the block that arrives last adds them up,
         // in their order.  No block waits for another.  The counter is 0 between launches.
         constexpr int kPairs = kMine / 2, kSlot = SETS * slot_floats(D) / 2;     // pairs of floats: of a lane, of a block
-        auto* const slot = reinterpret_cast<uint64_t*>(sums) + static_cast<int64_t>(blockIdx.x) * kSlot;
+        auto* const slot = reinterpret_cast<uint64_t*>(sums) + static_cast<int64_t>(it.id) * kSlot;
         const int at_sum = kPairs * 64 * kWaves + set * 16 + i;
         if (live) {
             #pragma unroll
@@ -370,13 +370,13 @@ __global__ __launch_bounds__(64 * kWaves, tree_blocks(KIND, D, PAGES16, SETS)) v
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        uint32_t* const counter = counters + (blockIdx.x - it.chunk * a.p.n_kv_heads);
+        uint32_t* const counter = counters + (it.id - it.chunk * a.p.n_kv_heads);
         if (tid == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if (uniform(arrived) + 1 != static_cast<uint32_t>(parts)) return;
         asm volatile("" ::: "memory");
         if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const uint64_t* const slots = reinterpret_cast<const uint64_t*>(sums) + static_cast<int64_t>(blockIdx.x - it.chunk * a.p.n_kv_heads) * kSlot;
+        const uint64_t* const slots = reinterpret_cast<const uint64_t*>(sums) + static_cast<int64_t>(it.id - it.chunk * a.p.n_kv_heads) * kSlot;
         const int64_t next = static_cast<int64_t>(a.p.n_kv_heads) * kSlot;
         auto pair_at = [&](int part, int at) {
             return __builtin_bit_cast(floatx2, __hip_atomic_load(slots + part * next + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));

@@ -259,3 +259,15 @@ def test_scales(queue, kind, scale):
                     if s[order[0]] - s[order[1]] > 20 + 2.0 ** -17 * np.abs(s[order[0]]):
                         want = v[order[0], h // 7]
                         assert (np.abs(got[c.start[b] + r, h] - want) <= 2.0 ** -9 * np.abs(want) + 2.0 ** -16).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(12, 6), (28, 7), (10, 5), (12, 12), (6, 3), (16, 8)])
+@pytest.mark.parametrize("lengths,new", [([2100], [50]), ([900, 33, 0, 1500], [40, 33, 0, 17]), ([70] * 70, [12] * 70)])
+def test_sets_of_rows_that_share_their_keys(queue, heads, kv_heads, lengths, new):
+    """Several sets of rows in several parts for numbers of key/value heads that do not go into eight, and in a batch of one; twice, as
+    the parts of a set meet in memory that the first call leaves ready for the next."""
+    c = TreeCache(mil.KV_F16, heads, kv_heads, 64, 16, lengths, new, seed=12).upload()
+    got = c.attend(queue)
+    c.check(got)
+    assert np.array_equal(got.view(np.uint16), c.attend(queue).view(np.uint16))
+    c.check(c.attend(queue, window=600, sinks=3), 600, 3)

@@ -49,6 +49,10 @@ extern "C" void items(const int* v, int room, int cus, const int* n, const int* 
         });
     }
 }
+extern "C" void apart(unsigned in, unsigned sets, unsigned pairs, unsigned* out) {
+    const SetOfPair x = eight_apart(in, sets, pairs);
+    out[0] = x.set, out[1] = x.pair;
+}
 extern "C" unsigned up(unsigned h) { return ascending(h); }
 extern "C" unsigned back(unsigned a) { return half_bits(a); }
 extern "C" int token(int tile, int lane, int e) { return token_of(tile, lane, e); }
@@ -151,3 +155,17 @@ def test_tiles_hold_every_token_once(rule):
     for beams, vocab in ((1, 1), (5, 200), (8, 151936), (64, 1 << 21)):
         n, room = rule.fit(16 << 20, beams, vocab), 136 * beams * rule.tiles(vocab)
         assert n * room <= 16 << 20 < (n + 1) * room and n >= 1
+
+
+def test_sets_of_a_pair_are_eight_blocks_apart(rule):
+    out = (ctypes.c_uint * 2)()
+    for sets in (1, 2, 3, 7, 16):
+        for pairs in (1, 2, 7, 8, 9, 15, 16, 40, 61):
+            where = {}
+            for i in range(sets * pairs):
+                rule.apart(i, sets, pairs, out)
+                where[out[0], out[1]] = i
+            assert sorted(where) == [(s, p) for s in range(sets) for p in range(pairs)]
+            for p in range(pairs):
+                step = 8 if p < pairs // 8 * 8 else pairs % 8
+                assert [where[s, p] - where[0, p] for s in range(sets)] == [s * step for s in range(sets)]
