@@ -57,11 +57,11 @@ constexpr int even_share(int share, int blocks, const Items& items) {
 // The sets of a sequence read the same keys.  Blocks go to the eight XCDs in turn, each with an L2 of its own: so that a part of the keys of a
 // key/value head (a pair) meets all its sets in one L2, they are eight blocks apart, one behind the other.  The sets and pairs of a sequence's blocks in
 // their order, block `in`; pairs behind the last whole eight lie side by side.
-// With the sets as far apart as a head has parts, key/value heads that do not go into eight spread them over all XCDs; and where one sequence is all there
-// is its sets read their keys at other times.  us for few rows (paged_tree.hip), that way / eight apart: 32 trees of 24, 15 heads over 5, behind 4096, fp16 38.7 /
-// 32.5; 8 of 16 behind 16384, 28 over 7, width 128 fp16 102 / 67, int8 61 / 50; 16 of 24 behind 4096, int8, 15 over 5 16.5 / 17.0 (the worst); one tree of 24
-// behind 16384, 12 over 6 25.6 / 18.0, 14 over 2 22.9 / 18.8, 32 over 8 22.0 / 19.5, width 128 47.2 / 47.5.  Else there is little in it: 16 of 24
-// behind 4096, int8, 14 over 2 15.0 / 16.0, 8 of 16 behind 16384 28.8 / 27.5.  For many rows (paged_tree_many.hip) nothing: 0.96 to 1.05.
+// With the sets as far apart as a head has parts it is chance whether they share an XCD, and key/value heads that do not go into eight spread them over
+// all; besides, they read their keys at other times.  us for few rows (paged_tree.hip), that way / eight apart: 32 trees of 24, 15 heads over 5, behind 4096, fp16
+// 38.7 / 32.5; 8 of 16 behind 16384, 28 over 7, width 128 fp16 102 / 67, int8 61 / 50; one tree of 24 behind 16384, 12 over 6 25.6 / 18.0, 14 over 2 22.9 / 18.8,
+// 32 over 8 22.0 / 19.5, width 128 47.2 / 47.5; 3 of 16 behind 9000, 32 over 8 23.2 / 19.3.  Over 576 cases of 1, 2, 4 and 8 key/value heads 0.82 to 1.07,
+// on average 0.99 of the time.  For many rows (paged_tree_many.hip) nothing: 0.96 to 1.05.
 struct SetOfPair {
     unsigned set, pair;
 };
@@ -74,7 +74,6 @@ constexpr SetOfPair eight_apart(unsigned in, unsigned sets, unsigned pairs) {
     const unsigned rest = pairs % 8, set = (in - whole) / rest;
     return {set, pairs / 8 * 8 + (in - whole - set * rest)};
 }
-constexpr bool eight_apart_pays(int n_seqs, int n_kv_heads) { return n_seqs == 1 || 8 % n_kv_heads != 0; }
 
 // Sets of rows_per_set rows that a launch over sequences of `from` to `to` rows has at most, whatever the lengths: every set full but
 // one of each sequence, of which there are no more than tokens and than times that `from` goes into all rows; and none longer than `to`.

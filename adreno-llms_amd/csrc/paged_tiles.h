@@ -198,7 +198,7 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
                 const unsigned heads = a.p.n_kv_heads;
                 it.id = blockIdx.x;
                 it.kvh = blockIdx.x - y * heads;
-                if (sets > 1 && eight_apart_pays(a.p.n_seqs, heads)) {
+                if (sets > 1) {
                     const SetOfPair x = eight_apart(own * heads + it.kvh, sets, n * heads);
                     it.set = x.set;
                     it.chunk = x.pair / heads;
