@@ -75,6 +75,11 @@ constexpr SetOfPair eight_apart(unsigned in, unsigned sets, unsigned pairs) {
     return {set, pairs / 8 * 8 + (in - whole - set * rest)};
 }
 
+// Tiles of 32 keys that a block is worth of a sequence that has so many (paged_tree.hip).
+constexpr int tree_worth(int tiles) {
+    return tiles <= 12 ? 12 : tiles <= 48 ? 4 : tiles <= 96 ? 8 : tiles <= 375 ? 16 : tiles <= 750 ? 32 : tiles <= 1500 ? 48 : 64;
+}
+
 // Sets of rows_per_set rows that a launch over sequences of `from` to `to` rows has at most, whatever the lengths: every set full but
 // one of each sequence, of which there are no more than tokens and than times that `from` goes into all rows; and none longer than `to`.
 constexpr int64_t sets_at_most(int64_t n_tokens, int64_t n_seqs, int nrep, int rows_per_set, int from, int to) {
@@ -221,7 +226,7 @@ constexpr PagedLaunches attention_launches(const AttentionSize& a, const Room& r
 //     16000 (500) 68 / 70 / 56; 32 of 256 at 2000 (1032) 106 / 93 / 87; 8 of 256 at 16384 (2064) fp16 265 / 194 / 116, int8 187 / 167 / 110.
 // Four sets of 16 rows to a wavefront spill registers and took 31 us for the 22.7 above.  At least 4 / 8 / 16 tiles to a block (4 wavefronts):
 // 112 rows at 916 (2) 6.8 / 7.6 / 8.8; 8 of 28 at 8000 (31) 15 / - / 9.8; 448 at 4096 (28) 14.5 / 11.5 / 11.5; 8 of 40 of 12 heads (107) 20.1 / - / 17.9.
-constexpr int kTreeFew = 64, kTreeTiny = 8, kTreeLittle = 16, kTreeMuch = 440;
+constexpr int kTreeFew = 64, kTreeLittle = 16, kTreeMuch = 440;
 constexpr PagedLaunch tree_launch(const AttentionSize& a, const Room& room, int64_t cus) {
     const int nrep = a.n_heads / a.n_kv_heads;
     const int64_t rows = static_cast<int64_t>(a.max_tokens) * nrep;
@@ -235,7 +240,7 @@ constexpr PagedLaunch tree_launch(const AttentionSize& a, const Room& room, int6
     const int sets = rows > kTreeFew && work > kTreeLittle * cus ? 2 : 1;
     const int64_t want = a.head_dim == 64 ? (sets == 1 ? 4 : 2) * cus : (sets == 1 ? 2 : 1) * cus;
     PagedLaunch l = make_launch(a, kRows * sets, 0, 0x7fffffff, want, room, sets * slot_floats(a.head_dim), 1);
-    l.plan.least = work > kTreeTiny * cus ? 4 * kWaves : kWaves;
+    l.plan.least = work > kTreeLittle * cus ? 4 * kWaves : 1;
     l.sets = sets;
     l.threads = 64 * kWaves;
     return l;

@@ -183,7 +183,8 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
     int before = 0;
     for (int b0 = 0;; ) {
         if (__any(down)) return it;
-        const int chunks = c.sets ? (c.tiles - 1) / it.share + 1 : 0, upto = scan(c.sets * chunks) + before;
+        const int worth = NEAR && plan.target > 0 ? tree_worth(c.tiles) : 0, share = it.share > worth ? it.share : worth;
+        const int chunks = c.sets ? (c.tiles - 1) / share + 1 : 0, upto = scan(c.sets * chunks) + before;
         const uint64_t past = __ballot(upto > y);
         if (past) {
             const int l = uniform(__builtin_ctzll(past));
@@ -204,14 +205,14 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
                     it.chunk = x.pair / heads;
                     it.kvh = x.pair - it.chunk * heads;
                     it.id = (y - own + x.set * n + it.chunk) * heads + it.kvh;
-                    if (n > 1) it.share = (it.tiles - 1) / n + 1;
+                    it.share = (it.tiles - 1) / n + 1;
                     return it;
                 }
             }
             const int set = sets == 1 ? 0 : own / n;
             it.chunk = own - set * n;
             it.set = sets - 1 - set;                                 // (the longest first)
-            if (n > 1) it.share = (it.tiles - 1) / n + 1;          // (the sequence's tiles in n equal parts)
+            if (NEAR || n > 1) it.share = (it.tiles - 1) / n + 1;          // (the sequence's tiles in n equal parts)
             return it;
         }
         before = __builtin_amdgcn_readlane(upto, 63);
