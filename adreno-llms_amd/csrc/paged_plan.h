@@ -75,6 +75,47 @@ constexpr SetOfPair eight_apart(unsigned in, unsigned sets, unsigned pairs) {
     return {set, pairs / 8 * 8 + (in - whole - set * rest)};
 }
 
+// The least share with which all items are no more than `blocks`, which are not fewer than the sets: items(share), fewer the greater it is, are at most
+// all / share + sets, and `most` leaves one per set.
+template <class Items>
+constexpr int fitting_share(float all, int sets, int blocks, int most, const Items& items) {
+    const float least = all / static_cast<float>(blocks), enough = blocks > sets ? all * 1.00001f / static_cast<float>(blocks - sets) + 1.0f : 1.0e9f;
+    int low = static_cast<int>(least * 0.99999f) - 1, share = enough < static_cast<float>(most) ? static_cast<int>(enough) : most;
+    if (low < 0) low = 0;                          // (not known to fit)
+    while (share - low > 1) {
+        const int mid = low + (share - low) / 2;
+        if (items(mid) <= blocks) share = mid;
+        else low = mid;
+    }
+    return share;
+}
+
+// The share for a launch of which a compute unit holds r blocks, one or two, and whose target is so many: by `share`, what share_of says, the last round of blocks
+// may be nearly empty.  Tried are the least shares that make one round and (r = 1) two, or (r = 2) one block for each unit; a tile's time is taken as
+// 3 + j where a unit has j blocks, a block's start and end as 12 tiles.  `blocks`: per key/value head of the launch, which items must not exceed.
+// us for few rows of width 128, with `share` / so: 4 trees of 64 behind 5474, 16 heads over 4, fp16 33.9 / 24.2; 8 of 32 behind 5165, 14 over 2, int8 29.9 / 21.9; 4 of 16
+// behind 13281, 32 over 8, fp16 46.6 / 38.4; 8 of 16 behind 34190, 8 over 1, int8 45.0 / 34.7; 8 of 64 behind 3494, 12 heads of their own, Q4 22.0 / 24.9 (the
+// worst).  At width 64, whose units hold two to four blocks, the same made 210 batches 3 % slower.
+template <class Items>
+constexpr int round_share(int share, float all, int sets, int most, const Plan& plan, int r, int blocks, const Items& items) {
+    const int unit = plan.target / r;
+    if (unit < 1) return share;
+    const auto time = [&](int j, int of) { return static_cast<float>(j <= r ? 3 + j : (3 + r) * ((j + r - 1) / r)) * static_cast<float>(of + 12); };
+    float best = 3.0e38f;
+    int found = share;
+    for (int k = 0; k < 2; ++k) {
+        const int j = k == 0 ? r : 3 - r, room = j * unit;
+        if (sets > room || room > blocks) continue;
+        const int least = fitting_share(all, sets, room, most, items), of = least < plan.least ? plan.least : least;
+        if (time(j, of) < best) {
+            best = time(j, of);
+            found = of;
+        }
+        if (all >= 0.85f * static_cast<float>(of) * static_cast<float>(room)) return found;
+    }
+    return time((items(share) + unit - 1) / unit, share) < best ? share : found;
+}
+
 // Tiles of 32 keys that a block is worth of a sequence that has so many (paged_tree.hip).
 constexpr int tree_worth(int tiles) {
     return tiles <= 12 ? 12 : tiles <= 48 ? 4 : tiles <= 96 ? 8 : tiles <= 375 ? 16 : tiles <= 750 ? 32 : tiles <= 1500 ? 48 : 64;

@@ -150,8 +150,9 @@ struct Item {
 //
 // EVEN: where a block's share is long, the least share is looked for with which the items still fit the launch's blocks: the first one leaves
 // a part of a share in the last part of each set, up to half of all (at 16 tiles and more: it takes about a microsecond).
-// NEAR: which of a sequence's items a block has is as eight_apart says, where that pays.
-template <int ROWS, int KEYS, bool EVEN = false, bool NEAR = false>
+// NEAR: which of a sequence's items a block has is as eight_apart says, and a part is what tree_worth says at least.  RESIDENT: shares are round_share's, for
+// that many blocks to a compute unit (where they are more than 16 tiles, with one to a unit 16, and not all that a sequence has: the search takes a microsecond).
+template <int ROWS, int KEYS, bool EVEN = false, bool NEAR = false, int RESIDENT = 0>
 __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan, const int y) {
     const int lane = threadIdx.x & 63;
     bool down = false;
@@ -180,10 +181,25 @@ __device__ __forceinline__ Item item_of(const AttentionArgs& a, const Plan& plan
             }));
         }
     }
+    if (RESIDENT > 0 && plan.target > 0 && it.share + (RESIDENT == 1) > 4 * kWaves && a.p.n_seqs <= 64 && __any(c.tiles > it.share)) {
+        const auto sum = [](float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sum_to_last(x)), 63)); };
+        const float sets = static_cast<float>(c.sets), tiles = static_cast<float>(c.tiles), worth = static_cast<float>(tree_worth(c.tiles));
+        const auto items = [&](int share) {        // (a tile's half: the quotient is no whole number that its rounding could miss)
+            return static_cast<int>(sum(sets * (floorf((tiles - 0.5f) * __builtin_amdgcn_rcpf(fmaxf(static_cast<float>(share), worth))) + 1.0f)));
+        };
+        const float most = wave_max(tiles);
+        if (most < 1.0e6f)
+            it.share = uniform(round_share(it.share, sum(sets * tiles), static_cast<int>(sum(sets)), static_cast<int>(most), plan, RESIDENT,
+                                           static_cast<int>(gridDim.x) / a.p.n_kv_heads, items));
+    }
     int before = 0;
     for (int b0 = 0;; ) {
         if (__any(down)) return it;
-        const int worth = NEAR && plan.target > 0 ? tree_worth(c.tiles) : 0, share = it.share > worth ? it.share : worth;
+        int share = it.share;
+        if constexpr (NEAR) {
+            const int worth = plan.target > 0 ? tree_worth(c.tiles) : 0;
+            if (share < worth) share = worth;
+        }
         const int chunks = c.sets ? (c.tiles - 1) / share + 1 : 0, upto = scan(c.sets * chunks) + before;
         const uint64_t past = __ballot(upto > y);
         if (past) {

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(64 * kWaves, tree_blocks(KIND, D, PAGES16, SETS)) v
     __shared__ uint32_t arrived;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const Item it = item_of<kRows * SETS, kKeys, false, true>(a, plan, blockIdx.x / a.p.n_kv_heads);
+    const Item it = item_of<kRows * SETS, kKeys, false, true, D == 64 ? 0 : SETS == 1 ? 2 : 1>(a, plan, blockIdx.x / a.p.n_kv_heads);
     if (it.b < 0) return;
     const int kvh = it.kvh;
     const int rows = it.s.n * plan.nrep, r0 = it.set * (kRows * SETS), r_end = r0 + kRows * SETS < rows ? r0 + kRows * SETS : rows;

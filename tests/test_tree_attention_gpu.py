@@ -271,3 +271,15 @@ def test_sets_of_rows_that_share_their_keys(queue, heads, kv_heads, lengths, new
     c.check(got)
     assert np.array_equal(got.view(np.uint16), c.attend(queue).view(np.uint16))
     c.check(c.attend(queue, window=600, sinks=3), 600, 3)
+
+
+@pytest.mark.parametrize("heads,kv_heads,lengths,new", [
+    (14, 2, [3000, 900, 2000], [30, 24, 9]), (32, 8, [2500] * 4, [32] * 4), (16, 4, [1700] * 5, [12] * 5), (8, 1, [4000, 1, 3900], [16, 1, 16]),
+    (12, 12, [2200, 700], [40, 3]), (14, 2, [1500] * 66, [4] * 66),
+])
+def test_rounds_of_blocks(queue, heads, kv_heads, lengths, new):
+    """Width 128, where blocks take a compute unit for themselves and shares of keys follow from the rounds that they make."""
+    c = TreeCache(mil.KV_INT8, heads, kv_heads, 128, 64, lengths, new, seed=13).upload()
+    got = c.attend(queue)
+    c.check(got)
+    assert np.array_equal(got.view(np.uint16), c.attend(queue).view(np.uint16))

@@ -49,6 +49,28 @@ extern "C" void items(const int* v, int room, int cus, const int* n, const int* 
         });
     }
 }
+// share, items: by share_of, then by round_share (sequences' sets and tiles; sums in fp32 as on the device, the quotients by a reciprocal that is `off` too great)
+extern "C" void rounds(int n, const int* sets, const int* tiles, int target, int resident, int least, int blocks, float off, int* out) {
+    Plan plan;
+    plan.target = target, plan.least = least;
+    float all = 0;
+    int every = 0, most = 0;
+    for (int b = 0; b < n; ++b) all += static_cast<float>(sets[b]) * static_cast<float>(tiles[b]), every += sets[b], most = tiles[b] > most ? tiles[b] : most;
+    const auto items = [&](int share) {
+        float sum = 0;
+        for (int b = 0; b < n; ++b) {
+            const float x = share > tree_worth(tiles[b]) ? share : tree_worth(tiles[b]);
+            sum += static_cast<float>(sets[b]) * (static_cast<float>(static_cast<int>((static_cast<float>(tiles[b]) - 0.5f) * (1.0f / x * off))) + 1.0f);
+        }
+        return static_cast<int>(sum);
+    };
+    int share = share_of(all, plan);
+    for (int pass = 0; pass < 2; ++pass, out += 2) {
+        out[0] = share, out[1] = 0;
+        for (int b = 0; b < n; ++b) out[1] += items_of({sets[b], tiles[b]}, share > tree_worth(tiles[b]) ? share : tree_worth(tiles[b]));
+        share = round_share(share, all, every, most, plan, resident, blocks, items);
+    }
+}
 extern "C" void apart(unsigned in, unsigned sets, unsigned pairs, unsigned* out) {
     const SetOfPair x = eight_apart(in, sets, pairs);
     out[0] = x.set, out[1] = x.pair;
@@ -169,3 +191,21 @@ def test_sets_of_a_pair_are_eight_blocks_apart(rule):
             for p in range(pairs):
                 step = 8 if p < pairs // 8 * 8 else pairs % 8
                 assert [where[s, p] - where[0, p] for s in range(sets)] == [s * step for s in range(sets)]
+
+
+def test_rounds_fit_the_launch(rule):
+    """A share by rounds of blocks never makes more items than the launch has blocks, and with one round or two where it says so."""
+    rng = random.Random(9)
+    better = 0
+    for _ in range(4000):
+        n, resident, kv = rng.choice([1, 2, 7, 32, 64]), rng.choice([1, 2]), rng.choice([1, 2, 3, 5, 8, 12])
+        sets = [rng.choice([0, 1, 2, 4, rng.randint(1, 30)]) for _ in range(n)]
+        tiles = [rng.choice([1, rng.randint(1, 40), rng.randint(1, 600), rng.randint(1, 30000)]) for _ in range(n)]
+        target = rng.choice([resident * 256 // kv, rng.randint(1, 300)])
+        least, blocks = rng.choice([1, 16]), target + sum(sets) + rng.choice([0, 0, 50])
+        out = (ctypes.c_int * 4)()
+        off = rng.choice([1.0, 1.0 + 2.0 ** -22, 1.0 - 2.0 ** -22])
+        rule.rounds(n, (ctypes.c_int * n)(*sets), (ctypes.c_int * n)(*tiles), target, resident, least, blocks, ctypes.c_float(off), out)
+        assert 1 <= out[2] and out[3] <= blocks and out[3] >= sum(sets), (sets, tiles, target, resident, list(out))
+        better += out[2] != out[0]
+    assert better > 1000
