@@ -136,6 +136,7 @@ struct AttentionSize {
     int n_seqs = 0, n_tokens = 0, max_tokens = 0, cap = 0;
     int n_heads = 1, n_kv_heads = 1, head_dim = 64;
     int window = 0, sinks = 0;
+    bool fp16 = true;         // the cache's kind, else int8 or Q4
 };
 struct Room {                 // of the stream's workspace: for sums, and counters
     size_t bytes = 0;
@@ -258,16 +259,24 @@ constexpr PagedLaunches attention_launches(const AttentionSize& a, const Room& r
 // Which kernel serves a call of mi_attention_tree, always one for the whole batch: the one for few rows with 16 rows of a tree (its drafts times
 // the heads of a group) per wavefront or with 32 (paged_tree.hip), or the one for many rows in blocks of 128 (paged_tree_many.hip).  The
 // first reads and converts the keys again for every 16 or 32 rows, the last has a chain of 1.3 us (width 128: 2.6) per tile of 64 keys.
-// us, 16 rows / 32 / 128, W: tiles of 16 rows by 32 keys per compute unit, by the host's bounds of rows and lengths:
-//   width 64: 1 tree of 112 rows at 916 (W 2) 7.0 / 8.7 / 12.7; 8 of 28 at 8000 (31) 9.8 / 11.8 / 20.8; 1 of 448 at 4096 (28) 12.8 / 11.5 / 21;
-//     8 of 40 of 12 heads of their own at 3000 (107) 18.1 / 20.3 / 21.9; 13 of 300 in a window of 1024, Q4 (174) 23.6 / 19.9 / 24.5;
-//     8 of 224 at 8192 (225) 22.4 / 18.1 / 25.2; 32 of 168 at 4096 (355) int8 24.9 / 22.7 / 25.1, fp16 33.7 / 25.6 / 25.3;
-//     32 of 280 at 3000, Q4 (427) 26.9 / 21.8 / 24.7; 8 of 448 at 8192 (451) 33.5 / 25.9 / 26.1; 32 of 448 at 2000 (451) 35.5 / 26.6 / 22.9.
-//   width 128: 1 of 64 at 16000 (62) 26.8 / 25.7 / 45; 16 of 48 at 4000 (189) 32 / 38 / 37.6; 1 of 256 at 16000 (251) 75 / 50 / 74; 8 of 64 at
-//     16000 (500) 68 / 70 / 56; 32 of 256 at 2000 (1032) 106 / 93 / 87; 8 of 256 at 16384 (2064) fp16 265 / 194 / 116, int8 187 / 167 / 110.
-// Four sets of 16 rows to a wavefront spill registers and took 31 us for the 22.7 above.  At least 4 / 8 / 16 tiles to a block (4 wavefronts):
-// 112 rows at 916 (2) 6.8 / 7.6 / 8.8; 8 of 28 at 8000 (31) 15 / - / 9.8; 448 at 4096 (28) 14.5 / 11.5 / 11.5; 8 of 40 of 12 heads (107) 20.1 / - / 17.9.
+// us, 16 rows / 32 / 128, W: tiles of 16 rows by 32 keys per compute unit, B: blocks of 128 rows, by the host's bounds of rows and lengths:
+//   width 64: 1 tree of 112 rows at 916 (W 2) 7.0 / 8.7 / 12.7; 2 of 100 at 2372, int8 (49) 11.3 / 13.4 / 18.8; 4 of 400 at 914 (45) 12.2 / 11.0 / 17.2; 4 of 300
+//     at 6949, Q4 (194) 24.2 / 22.0 / 31.7; 32 of 168 at 4096 (355) int8 24.9 / 22.7 / 25.1, fp16 33.7 / 25.6 / 25.3; 32 of 192 at 2367 (333, B 192) fp16
+//     37.1 / 29.3 / 24.6; 8 of 400 at 4015, Q4 (788) 48.9 / 34.2 / 35.0; 32 of 300 at 2696 (606) 54 / 43 / 32.5.
+//   width 128: 4 of 96 at 3710, Q4 (49) 15.8 / 19.1 / 29; 1 of 400 at 5044 (64) 26.4 / 23.9 / 42; 4 of 96 at 5793, Q4 (54) 18.3 / 19.7 / 34.7; 8 of 512 at 3600 (77)
+//     21.4 / 19.5 / 30.7; 1 of 256 at 8519 (136) fp16 45.8 / 33.9 / 53.7; 4 of 400 at 1883 (136) int8 29.4 / 37.8 / 32.6; 8 of 512 at 7286 (152) 32.0 / 25.7 / 46.2;
+//     16 of 512 at 5548, Q4 (241) 39.0 / 41.6 / 50.0; 16 of 256 at 2083, int8 (196, B 144) 34.5 / 44.2 / 35.0; 8 of 400 at 4558 (303, B 92) 72 / 55 / 45.8; 2 of 128 at
+//     24969, int8 (294, B 24) 59 / 52 / 71; 32 of 192 at 2276 (409, B 310) 114 / 84 / 45; 8 of 224 at 27113 (525, B 32) 88 / 64 / 97; 16 of 128 at 5583 (542, B 208)
+//     91 / 79 / 51.
+// Over 150 batches of each width (W 16 or 40 to 700) this takes 1.01 and 1.02 times the best of the three.  Four sets of 16 rows to a wavefront spill registers
+// and took 31 us for the 22.7 above.  In batches of more than little work a block has 16 tiles at least, whatever tree_worth says: 16 trees of 16 of 15 heads over 5 behind
+// 1203, int8 10.2, with 8 11.2; 4 of 2 of 12 heads of their own, width 128, behind 3432 13.7 and 17.7.
 constexpr int kTreeFew = 64, kTreeLittle = 16, kTreeMuch = 440;
+// W up to which 16 rows to a wavefront are better, and from which 128 are if there are blocks for a part of the units.
+constexpr int one_set_up_to(int D, bool fp16) { return D == 64 ? fp16 ? 30 : 60 : fp16 ? 60 : 250; }
+constexpr bool blocks_enough(int D, bool fp16, int64_t work, int64_t blocks, int64_t cus) {
+    return work > 250 * cus && (D == 128 ? 4 * blocks >= cus : fp16 && 2 * blocks >= cus);
+}
 constexpr PagedLaunch tree_launch(const AttentionSize& a, const Room& room, int64_t cus) {
     const int nrep = a.n_heads / a.n_kv_heads;
     const int64_t rows = static_cast<int64_t>(a.max_tokens) * nrep;
@@ -277,8 +286,10 @@ constexpr PagedLaunch tree_launch(const AttentionSize& a, const Room& room, int6
         if (seen < keys) keys = seen;
     }
     const int64_t work = sets_at_most(a.n_tokens, a.n_seqs, nrep, kRows, 0, 0x7fffffff) * a.n_kv_heads * (keys / kKeys + 1);
-    if (work > kTreeMuch * cus && rows > kRows) return slices_launch(a, room, 4, 1, 0, 2 * cus);
-    const int sets = rows > kTreeFew && work > kTreeLittle * cus ? 2 : 1;
+    const int64_t many = sets_at_most(a.n_tokens, a.n_seqs, nrep, 128, 0, 0x7fffffff) * a.n_kv_heads;
+    if ((work > kTreeMuch * cus && rows > kRows) || (rows > kTreeFew && blocks_enough(a.head_dim, a.fp16, work, many, cus)))
+        return slices_launch(a, room, 4, 1, 0, 2 * cus);
+    const int sets = rows > kTreeFew && work > one_set_up_to(a.head_dim, a.fp16) * cus ? 2 : 1;
     const int64_t want = a.head_dim == 64 ? (sets == 1 ? 4 : 2) * cus : (sets == 1 ? 2 : 1) * cus;
     PagedLaunch l = make_launch(a, kRows * sets, 0, 0x7fffffff, want, room, sets * slot_floats(a.head_dim), 1);
     l.plan.least = work > kTreeLittle * cus ? 4 * kWaves : 1;

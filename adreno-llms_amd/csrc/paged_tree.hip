@@ -453,7 +453,8 @@ bool launch_sets(hipStream_t s, const TreeArgs& a, float* sums, uint32_t* counte
 
 bool launch_paged_tree(hipStream_t s, const TreeArgs& a, const StreamRoom& own) {
     const bool room = own.workspace && own.sums;
-    const AttentionSize size = {a.p.n_seqs, a.p.n_tokens, a.max_tokens, a.p.cap, a.n_heads, a.p.n_kv_heads, a.head_dim, a.window, a.sinks};
+    const AttentionSize size = {a.p.n_seqs, a.p.n_tokens, a.max_tokens, a.p.cap, a.n_heads, a.p.n_kv_heads, a.head_dim, a.window, a.sinks,
+                                a.kind == MI_KV_F16};
     PagedLaunches all;
     all.n = 1;
     const PagedLaunch& l = all.of[0] = tree_launch(size, room ? Room{kPartialBytes, kSliceCounters} : Room{}, device_info().cus);
