@@ -20,6 +20,7 @@ def queue():
 
 
 COLUMNS = [0, 2 ** 14, 2 ** 20]
+WIDER = 2 ** 16
 
 
 @pytest.fixture(autouse=True, params=COLUMNS, ids=["tight", "middle", "wide"])
@@ -50,6 +51,16 @@ def test_against_64_bits(queue, kind, case):
     c = TreeCache(kind, seed=1, **case).upload()
     c.check(c.attend(queue))
     c.check(c.attend(queue, ld_out=c.heads * c.D + 5), what="rows apart")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("case", [CASES[6], CASES[8]])
+def test_wider_tables(queue, kind, case, monkeypatch):
+    """Codes of width 128 come to 32 rows to a wavefront under tables for more positions than fp16."""
+    monkeypatch.setattr(Cache, "columns", WIDER)
+    c = TreeCache(kind, seed=6, **case).upload()
+    c.check(c.attend(queue))
+    c.check(c.attend(queue, window=50, sinks=2), 50, 2)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (33, 0), (100, 37), (2 ** 31 - 1, 2 ** 31 - 1)])

@@ -17,7 +17,7 @@ DRIVER = """
 using namespace mi;
 static const Room kAll{32u << 20, 16384};
 static PagedLaunch launch_of(const int* v, int room, int cus) {
-    return tree_launch(AttentionSize{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8]}, room ? kAll : Room{}, cus);
+    return tree_launch(AttentionSize{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9] == 0}, room ? kAll : Room{}, cus);
 }
 // wavefronts, slices, sets, target, blocks per key/value head, threads
 extern "C" void launch(const int* v, int room, int cus, int* out) {
@@ -81,7 +81,7 @@ extern "C" int token(int tile, int lane, int e) { return token_of(tile, lane, e)
 extern "C" int tiles(int vocab) { return tiles_of_row(vocab); }
 extern "C" long long fit(long long bytes, int beams, int vocab) { return groups_that_fit(bytes, beams, vocab); }
 """
-NAMES = "n_seqs n_tokens max_tokens cap n_heads n_kv_heads head_dim window sinks".split()
+NAMES = "n_seqs n_tokens max_tokens cap n_heads n_kv_heads head_dim window sinks codes".split()
 
 
 @pytest.fixture(scope="module")
@@ -97,7 +97,7 @@ def rule(tmp_path_factory):
     lib.fit.restype, lib.fit.argtypes = ctypes.c_longlong, [ctypes.c_longlong, ctypes.c_int, ctypes.c_int]
 
     def size(s):
-        return (ctypes.c_int * 9)(*[s.get(n, 0) for n in NAMES])
+        return (ctypes.c_int * 10)(*[s.get(n, 0) for n in NAMES])
 
     def launch(s, room=True, cus=256):
         out = (ctypes.c_int * 6)()
@@ -131,6 +131,7 @@ def test_blocks_suffice(rule):
         s = size_of(new, lengths, heads, kv, D, pad=rng.choice([0, 0, 33, 4000]), window=rng.choice([0, 0, 100, 1000]), sinks=rng.choice([0, 4]))
         if rng.random() < 0.2:
             s["max_tokens"] = rng.choice([0, 1, 7, 5000])                          # a wrong hint
+        s["codes"] = rng.choice([0, 1])
         room = rng.random() < 0.8
         l = rule.launch_of(s, room)
         assert l["threads"] == 64 * (l["wavefronts"] or 4) and l["slices"] == 1
@@ -145,14 +146,16 @@ def test_blocks_suffice(rule):
 
 def test_cases_come_to_the_kernels_that_they_are_for(rule):
     """On 256 compute units, those of the device that they are written for."""
-    from test_tree_attention_gpu import CASES, COLUMNS
+    from test_tree_attention_gpu import CASES, COLUMNS, WIDER
 
-    seen = set()
-    for case in CASES:
-        for columns in COLUMNS:
-            l = rule.launch_of(size_of(case["new"], case["lengths"], case["heads"], case["kv_heads"], case["D"], case.get("pad", 0), case["page"], columns))
-            seen.add((case["D"], case["page"] % 16 == 0, l["wavefronts"], l["sets"]))
-    assert seen == {(D, whole, w, s) for D in (64, 128) for whole in (True, False) for w, s in ((0, 1), (0, 2), (4, 1))}, seen
+    for codes in (0, 1):                                                           # fp16; int8 or Q4
+        seen = set()
+        for case in CASES:
+            for columns in COLUMNS + [WIDER] * (case is CASES[8]):
+                l = rule.launch_of(size_of(case["new"], case["lengths"], case["heads"], case["kv_heads"], case["D"], case.get("pad", 0), case["page"], columns,
+                                           codes=codes))
+                seen.add((case["D"], case["page"] % 16 == 0, l["wavefronts"], l["sets"]))
+        assert seen == {(D, whole, w, s) for D in (64, 128) for whole in (True, False) for w, s in ((0, 1), (0, 2), (4, 1))}, (codes, seen)
 
 
 def test_halves_ascend(rule):
