@@ -116,7 +116,12 @@ constexpr int round_share(int share, float all, int sets, int most, const Plan& 
     return time((items(share) + unit - 1) / unit, share) < best ? share : found;
 }
 
-// Tiles of 32 keys that a block is worth of a sequence that has so many (paged_tree.hip).
+// Tiles of 32 keys that a block is worth of a sequence that has so many (paged_tree.hip): fewer are a shorter chain of tiles, more are fewer parts for a set's last
+// block to add up, about a microsecond for eight.  us at 4 / 8 / 16 / 32 / 48 tiles, one tree of 4 of 14 heads over 2, width 64, fp16: behind 150 positions 7.2 / 6.8 /
+// 6.5 / - / -; 1000 7.4 / 7.7 / 9.0 / 9.8; 2000 8.2 / 7.6 / 8.9 / 11.6; 4000 9.8 / 8.7 / 8.7 / 11.3; 8000 13.7 / 10.4 / 9.5 / 11.1; 16000 21.1 / 14.0 / 11.5 / 12.1.
+// Batches of 8 to 32 and 32 to 100 tiles of 16 rows to a compute unit, times the best: 2000 1.23 / 1.04 / 1.09 / 1.41 and 1.22 / 1.11 / 1.05 / 1.30; 8000 1.45 / 1.22 /
+// 1.01 / 1.12 and 1.23 / 1.19 / 1.11 / 1.07; 16000 1.61 / 1.35 / 1.07 / 1.02 and 1.35 / 1.30 / 1.17 / 1.01; 32000 1.93 / 1.56 / 1.17 / 1.02 / 1.06 and 1.35 / 1.31 /
+// 1.22 / 1.07 / 1.08.
 constexpr int tree_worth(int tiles) {
     return tiles <= 12 ? 12 : tiles <= 48 ? 4 : tiles <= 96 ? 8 : tiles <= 375 ? 16 : tiles <= 750 ? 32 : tiles <= 1500 ? 48 : 64;
 }

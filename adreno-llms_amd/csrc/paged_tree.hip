@@ -6,10 +6,10 @@
 // wavefront streams its tiles of 32 keys from memory to the operands of the matrix instructions, without LDS or barriers as the kernel
 // for few rows of a plain batch does, and multiplies each of them with SETS times 16 rows.
 //
-// What bounds it: launch, planning, queries and the meeting of parts, about 7 us whatever the lengths (16 drafts of 14 heads over 2 behind 900: 6.8);
+// What bounds it: launch, planning, queries and the meeting of parts, about 7 us whatever the lengths (16 drafts of 14 heads over 2 behind 900: 7.0);
 // beyond, the vector units and the wait for the next tile share a tile's time: with two sets in int8 a tile is 290 vector
 // instructions, 32 of them exponentials, 60 scalar ones and 24 matrix products, 0.6 us of a SIMD with three wavefronts that take 1.0.  32 trees of 24
-// drafts behind 4096, int8 22.4 us; 13 of 100 in a window of 1024, Q4, pages of 48 19.8.
+// drafts behind 4096, int8 22.5 us; 13 of 100 in a window of 1024, Q4, pages of 48 20.2.
 #include "paged_tiles.h"
 
 namespace mi {
