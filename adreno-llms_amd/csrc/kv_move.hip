@@ -175,7 +175,7 @@ __global__ __launch_bounds__(kCopyThreads) void kv_reorder_kernel(const ReorderA
 bool off(const void* p, uintptr_t align) { return !p || reinterpret_cast<uintptr_t>(p) % align; }
 
 // Checks the caches of a call, which are alike but for their pools, and its batch.  (A pool that is there twice would have its rows moved twice,
-// by two wavefronts at once.  Every pool is compared with all before it: half a microsecond for 32 caches.)
+// by two wavefronts at once.  Every pool is compared with all before it: for 24 caches nothing that shows beside the call, 7.65 us with and without.)
 bool layers_args(const char* who, const mi_kv_cache* caches, int n, const mi_kv_batch& batch, PagedArgs* out) {
     if (!caches || n < 1) {
         MI_ERROR_FMT("%s: no caches (caches=%p n_caches=%d)", who, static_cast<const void*>(caches), n);
