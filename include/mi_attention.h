@@ -140,7 +140,8 @@ int mi_attention_tree(void* stream, const mi_attention_call* call, const mi_tree
  * n_b earlier positions, the rows numbered keep[q_start[b] + i], i = 0 .. kept[b] - 1, ascending, each of 0 .. n_b - 1, become
  * positions before + i, in every cache of `caches`; what the other positions hold is left as it is.  new_len[b] = before + kept[b] (kept
  * taken as within 0 .. n_b; less than 0 counts as 0) unless new_len is null; it overlaps none of the arrays that are read.
- * caches: n_caches of them, the layers of a model say, which differ in their pools alone; no pool is there twice.  keep [n_tokens] (what lies behind a
+ * caches: n_caches of them, the layers of a model say, which differ in their pools alone; no pool is there twice, nor, of int8 and Q4 caches, one of
+ * scales.  keep [n_tokens] (what lies behind a
  * sequence's kept ones is not read), kept [n_seqs], new_len [n_seqs]: device memory, 4-byte aligned.  Rows move as they are stored.  A row
  * or a place that is not in the cache, or a number out of range, moves nothing.  Where numbers do not ascend it is not said
  * which rows end up where, but no other positions are touched.  No two sequences of a call share a page that holds a new row. */
@@ -152,7 +153,7 @@ int mi_kv_keep(void* stream, const mi_kv_cache* caches, int n_caches, const mi_k
  * kv_len[f] % page_size rows are copied, in every cache of `caches`, to page fresh[b], which takes its place (f = b keeps its own and fresh[b] is
  * not used).  Full pages are shared from then on, which the host counts.  source[b] outside 0 .. n_seqs - 1: new_len[b] = 0, all
  * pages -1.  kv_len[f] beyond the table, or a page (old or fresh) that is not in the pool: the number is passed on, nothing is copied.
- * A fresh page is nobody's: neither in `pages` nor twice in `fresh` among those that are used.  kv_len, source, fresh, new_len
+ * `caches` as for mi_kv_keep.  A fresh page is nobody's: neither in `pages` nor twice in `fresh` among those that are used.  kv_len, source, fresh, new_len
  * [n_seqs], pages, new_pages [n_seqs][max_pages]: device memory, 4-byte aligned; new_len and new_pages overlap none of the others. */
 typedef struct mi_kv_reorder_call {
     const int *kv_len, *pages, *source, *fresh;
