@@ -2,9 +2,8 @@
 // pair, between a batch's projections and its cache.  (The decoders' own rotary embedding, with its tables of rounded cosines, is
 // in decode.hip.)
 //
-// An angle of position 10^6 is known to 2^-4 in fp32, so it is taken in 64 bits, in turns: position * inv_freq / 2 pi less the
-// nearest integer is within 2^-22 of a turn for any position (2^31 of them, three roundings of 2^-53), and its cosine and sine are
-// fp32's.  All heads of a row turn by the same angles, which a wavefront works out once, a pair per lane, and hands round in LDS.
+// An angle of position 10^6 is known to 2^-4 in fp32, so it is taken in 64 bits and what their roundings leave, in turns (rope_rule.h), and its cosine
+// and sine are fp32's.  All heads of a row turn by the same angles, which a wavefront works out once, a pair per lane, and hands round in LDS.
 //
 // What bounds it: bytes where there are many rows, 84 MB of 4096 rows of 32 + 8 heads of 128 in 14.3 us (16.4 with rows that no cache holds, a
 // large copy's rate); below about 2000 rows the host's call (6.5 us; on the GPU 16 rows 3.3: the launch, the positions, the angles).  An
@@ -12,6 +11,7 @@
 #include "../../include/mi_attention.h"
 #include "common.h"
 #include "device_math.h"
+#include "rope_rule.h"
 
 namespace mi {
 namespace {
@@ -35,9 +35,7 @@ struct RopeArgs {
 __device__ __forceinline__ void angles(const RopeArgs& a, int row, int lane, float* turn) {
     for (int i = lane; i < a.pairs; i += 64) {
         const int axis = a.axis[i / 16] >> (i % 16 * 2) & 3;
-        const double p = a.position[static_cast<int64_t>(axis) * a.n_tokens + row];
-        const double t = p * static_cast<double>(a.inv_freq[i]) * 0.15915494309189533577;      // 1 / 2 pi
-        const float f = 2.0f * static_cast<float>(t - rint(t));
+        const float f = 2.0f * static_cast<float>(turns_of<>(a.position[static_cast<int64_t>(axis) * a.n_tokens + row], a.inv_freq[i]));
         turn[i] = cospif(f);
         turn[kMostPairs + i] = sinpif(f);
     }

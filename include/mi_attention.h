@@ -103,8 +103,8 @@ int mi_attention(void* stream, const mi_attention_call* call);
  *               null).  fp16, 2-byte aligned.  An output may be its own input, with the same ld; else outputs overlap nothing.
  *   position    int32 [n_axes][n_tokens], inv_freq fp32 [rot_dim / 2]: device memory.
  *   axis        host memory, read during the call: of each i the number of its axis; null: all 0.
- * head_dim even, up to 256; rot_dim even, 0 to head_dim; n_axes 1 to 4.  The angle is taken in 64 bits and cosine and sine to fp32's last
- * bits at any position; an output is rounded to fp16 once.  The reference has one axis, the halves' pairs and fp16 tables
+ * head_dim even, up to 256; rot_dim even, 0 to head_dim; n_axes 1 to 4.  The angle is taken in 64 bits and what their roundings
+ * leave, so that cosine and sine are right to fp32's last bits at any position; an output is rounded to fp16 once.  The reference has one axis, the halves' pairs and fp16 tables
  * (QW/kernels/rope.cl, QW/src/layers/attention.cpp:133-172), as mi_decoder_step keeps them. */
 typedef struct mi_rope_call {
     const void *q, *k;
