@@ -147,14 +147,17 @@ int mi_linear_argmax_static(void* stream, int N, int K, const void* x, const voi
  * of logits (fp16 [n_groups * beams], ld elements apart, `vocab` of them) and score (fp32, the sum of log probabilities so far) are group
  * g's.  Its n_out best continuations are left, best first, in out_score, out_token and out_row [n_groups][n_out]: token t of row r counts
  *   score[r] + logits[r][t] - log sum_u exp logits[r][u],
- * compared in 64 bits and left as fp32; among equals the lowest row, then the lowest token (scores up to 2^28 in size: beyond, the sums
- * of one row's different logits are equal).  -infinity is a logit that is never chosen (a
+ * added and compared in 64 bits and left as fp32; among equals the lowest row, then the lowest token (scores up to 2^28 in size: beyond, the
+ * sums of one row's different logits are equal).  The exponentials and their sums are fp32's, 4096 logits at a time, so the logarithm is off by some 2^-23, at
+ * most 2^-20: rows that hold the same logits in the same places are equal, but those whose true sums are nearer than that, the same logits in another
+ * order for one, come in either order.  -infinity is a logit that is never chosen (a
  * token that a grammar forbids); a row whose score is not finite (a beam that is not there, the others of a first step), whose
  * logits are all -infinity, or that holds a NaN or +infinity is never chosen from.  Where fewer than n_out are left the others are
  * -infinity, -1, -1.  out_row is a number of all rows, as mi_kv_reorder takes it.  With n_out = 2 * beams a host has enough whichever
  * of them end.  The reference decodes greedily or samples; it has no beams.
  * The outputs overlap nothing.  beams and n_out 1 to 64, vocab up to MI_BEAM_MAX_VOCAB.  Two launches on a stream of mi_stream_create or the null stream, whose
- * workspace holds the rows' sums and maxima in between; on any other stream one launch, slower.  Nothing is allocated or waited for. */
+ * workspace holds the rows' sums and maxima in between (two for as many groups as fit, about 16 MB / (136 bytes * rows * tiles of 4096 logits));
+ * on any other stream one launch, slower.  Nothing is allocated or waited for. */
 #define MI_BEAM_MAX_VOCAB (1 << 21)
 typedef struct mi_beam_call {
     const void* logits;
