@@ -3,12 +3,13 @@
 // One pass over the logits: a wavefront has a tile of 4096 in registers, takes the sum of their exponentials relative to the tile's
 // greatest and the greatest of each lane's 64 (a bin), a 64th of what it read.  A row's best n_out then lie in bins that reach the
 // n_out-th greatest of a wavefront's maxima over all bins, some 20 of 2400, which are read again.  Within a row the order is that of the
-// fp16 logits themselves, ties by token; rows of a group are merged by sums in 64 bits, which a near tie of two beams turns on.
+// fp16 logits themselves, ties by token; rows of a group are merged by sums in 64 bits, of which a row's logarithm has the
+// error of fp32's exponentials.
 //
 // What bounds it: the pass over many logits by memory, 78 MB of 256 rows of 151 936 in 14.2 us, 5.4 TB/s (an exponential takes 16 cycles of a
 // SIMD, a logit 26 in all: 7 us of the vector units); behind it, and for few rows, a chain that a group's block goes through once: 5 us for 4 rows, 7.5
 // for 8 rows by 32 groups, of which two answers of memory (bins, logits) are 1.5 and 2.9 and the rest instructions of one
-// wavefront, eight cycles each.  Before offers that share a place were told apart among themselves it was 11 for 8 rows; with candidates in
+// wavefront, eight cycles each; rows of one or two tiles: see pick_crowded.  Before offers that share a place were told apart among themselves it was 11 for 8 rows; with candidates in
 // order and merged one list after the other 7 and 14; with calls of functions, which need scratch memory, 9 and 24.  Error of the sum: 3e-8 of a score near -20.
 #include "../../include/mi_linear.h"
 #include "beam_rule.h"
@@ -201,8 +202,11 @@ __device__ __forceinline__ uint32_t reach(ushort8 x, uint32_t below) {
     return (w[0] | w[1] << 1) | (w[2] | w[3] << 1) << 2;
 }
 
-// The best n of a row's logits, in order, where so many reach `least` that the fast way has no room for them (values that tie, mostly): bin
-// after bin, the best kept whenever the list is full; bins that cannot hold a better one are passed over.
+// The best n of a row's logits, in order, where so many reach `least` that the fast way has no room for them: bin after bin, each an answer of
+// memory, the best kept whenever the list is full; bins that cannot hold a better one are passed over.  So it is where many values tie, and where
+// few lanes have bins: a lane holds eight neighbouring ones, so a tile has them in eight lanes, and `least` is below all logits for more outputs
+// than that (up to 24; beyond, than four times as many).  4 beams of 4096 tokens: 8 outputs 9.4 us, 9 36.8, 25 10.7, 64 52; 10 beams, 20 outputs: 1000 tokens 57,
+// 8000 84, 12000 17.
 __device__ __forceinline__ int pick_crowded(const uint16_t* row, int vocab, int all, const uint16_t* bins, int n, uint32_t least, PickRoom& room) {
     const int lane = threadIdx.x & 63;
     uint64_t above = static_cast<uint64_t>(least) << 32;
@@ -244,7 +248,8 @@ __device__ __forceinline__ int pick(const uint16_t* row, int vocab, int tiles, c
             }
         }
     };
-    // n of the lanes' maxima, over all of their bins or (many wanted) over a quarter of them each, reach `least`, so the best n candidates do
+    // n of the lanes' maxima, over all of their bins or (many wanted) over a quarter of them each, reach `least`, so the best n candidates do (no n lanes
+    // with bins: all do)
     ushort8 top = {};
     #pragma unroll 1
     for (int from = (all - 1) / kAtOnce * kAtOnce; from >= 0; from -= kAtOnce) {

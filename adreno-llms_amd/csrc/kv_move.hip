@@ -26,7 +26,7 @@ struct Layers {
 //
 // What bounds it: five trips to memory one after the other, to lengths, numbers, page table, rows and back, and the launch: 16 paths in 24 layers of
 // 2 x 64 3.8 to 4.2 us on the GPU, 7.6 with the host's call; 48 paths of up to 11 rows in 16 layers of 8 x 128, 17 MB, 8.1 to 8.9 (each row's
-// place looked up where it moves, four rows at a time: 10).
+// place looked up where it moves, four rows at a time: 10).  In int8 and Q4 all of these are the host's call, 7.4 to 8.2.
 constexpr int kAhead = 8;
 
 struct KeepArgs {
@@ -108,7 +108,8 @@ __global__ __launch_bounds__(64) void kv_keep_kernel(const KeepArgs a, const Lay
 // ---- copies of sequences ----------------------------------------------------------------------------------
 //
 // The rows of a last page lie together for each head, and go in pieces of 16 bytes; the tables go in the same launch.  What bounds it: bytes where
-// there are many, 48 beams' pages of up to 99 rows of 8 x 128 in 16 layers, 180 MB written, 67 to 70 us (copies of one page read it from the caches);
+// there are many, 48 beams' pages of up to 99 rows of 8 x 128 in 16 layers, 180 MB written, 67 to 70 us (copies of one page read it from the caches), of int8
+// and Q4 33 and 21, as many bytes a second (their scales go by two bytes a thread);
 // else the launch and three trips, 2.7 to 3.1 us on the GPU for 16 beams in 24 layers, 7.3 with the host's call.
 
 struct ReorderArgs {

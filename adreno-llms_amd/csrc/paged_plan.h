@@ -95,7 +95,7 @@ constexpr int fitting_share(float all, int sets, int blocks, int most, const Ite
 // 3 + j where a unit has j blocks, a block's start and end as 12 tiles.  `blocks`: per key/value head of the launch, which items must not exceed.
 // us for few rows of width 128, with `share` / so: 4 trees of 64 behind 5474, 16 heads over 4, fp16 33.9 / 24.2; 8 of 32 behind 5165, 14 over 2, int8 29.9 / 21.9; 4 of 16
 // behind 13281, 32 over 8, fp16 46.6 / 38.4; 8 of 16 behind 34190, 8 over 1, int8 45.0 / 34.7; 8 of 64 behind 3494, 12 heads of their own, Q4 22.0 / 24.9 (the
-// worst).  At width 64, whose units hold two to four blocks, the same made 210 batches 3 % slower.
+// worst: what tells such a batch from the others beforehand is not known).  At width 64, whose units hold two to four blocks, the same made 210 batches 3 % slower.
 template <class Items>
 constexpr int round_share(int share, float all, int sets, int most, const Plan& plan, int r, int blocks, const Items& items) {
     const int unit = plan.target / r;

@@ -7,9 +7,11 @@
 // for few rows of a plain batch does, and multiplies each of them with SETS times 16 rows.
 //
 // What bounds it: launch, planning, queries and the meeting of parts, about 7 us whatever the lengths (16 drafts of 14 heads over 2 behind 900: 7.0);
-// beyond, the vector units and the wait for the next tile share a tile's time: with two sets in int8 a tile is 290 vector
-// instructions, 32 of them exponentials, 60 scalar ones and 24 matrix products, 0.6 us of a SIMD with three wavefronts that take 1.0.  32 trees of 24
-// drafts behind 4096, int8 22.5 us; 13 of 100 in a window of 1024, Q4, pages of 48 20.2.
+// beyond, the vector units and the wait for memory.  With two sets in int8 a tile that all rows see is 194 vector instructions, 16 of them
+// exponentials, 100 scalar ones and 16 matrix products; a launch has 273 and 159 for each tile, planning, queries, masks and sums counted in.  Counters
+// of 32 trees of 24 drafts behind 4096, int8, 22.5 us: vector units busy 54 % of the SIMD-cycles, matrix cores 11 %; of the wavefronts' time, 2.3 to
+// a SIMD, 40 % are instructions, 34 % waits for memory (a tile's keys are asked for behind the last one's key products, its values
+// behind its value products) and 26 % for their turn.  13 of 100 in a window of 1024, Q4, pages of 48, 20.2 us: 54 %, 8 %; 2.5 to a SIMD, 36, 40 and 24 %.
 #include "paged_tiles.h"
 
 namespace mi {
@@ -25,9 +27,9 @@ __device__ __forceinline__ float sum_of_groups(float a) {
 }
 
 constexpr int tree_lds(int D, int SETS) { return kWaves * SETS * (D / 4 + 2) * 64 * 4; }
-// Blocks to a compute unit that the registers have to do for.  Two sets of width 64 in pages of whole sixteens: three, with 22 registers
+// Blocks to a compute unit that the registers have to do for.  Two sets of width 64 in pages of whole sixteens: three, with 11 registers
 // spilled in fp16 (32 trees of 24 drafts behind 4096 positions 25.6 us, with two 28.8; int8 and Q4 spill none), else two; of width 128
-// one (two spill a hundred registers).
+// one (264 to 320 registers, no spills, but 48 bytes of scratch memory: the division by nrep in the end is a call there, which takes the plan by its address).
 constexpr int tree_blocks(int KIND, int D, bool PAGES16, int SETS) {
     if (D == 128) return SETS == 1 ? 2 : 1;
     return SETS == 2 ? PAGES16 ? 3 : 2 : KIND == MI_KV_F16 && !PAGES16 ? 3 : 4;

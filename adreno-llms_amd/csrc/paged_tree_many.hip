@@ -1,6 +1,7 @@
 // Attention of trees of many rows over a cache in pages (mi_attention_tree): the kernel for many rows, in a file of its own so that
-// both compile at the same time.  8 trees of 64 drafts behind 16384, 32 heads over 8 of width 128: fp16 109 us, int8 103, Q4 107 (matrix cores busy 25 % of
-// the SIMD-cycles, vector units 29 %, LDS 38 % of the CU-cycles, a third of it conflicts: the chain of a tile, as in plain batches).
+// both compile at the same time.  8 trees of 64 drafts behind 16384, 32 heads over 8 of width 128: fp16 108 us, int8 103, Q4 107.  What bounds it is the chain
+// of a tile, as in plain batches; counters of the fp16 ones: matrix cores busy 29 % of the SIMD-cycles, vector units 33 %, LDS 30 % of the CU-cycles (half of it
+// conflicts); of the wavefronts' time 40 % are instructions, 37 % waits for memory, LDS and barriers, 23 % for their turn.
 #include "paged_chunk.h"
 
 namespace mi {

@@ -113,7 +113,8 @@ __global__ __launch_bounds__(64 * kWaves) void rope_wide_kernel(const RopeArgs a
     }
 }
 
-// The same for any rows, a lane one pair after the other.
+// The same for any rows, a lane one pair after the other, two bytes a load: rows that begin, or lie apart, at other than multiples of 16 bytes,
+// heads or turned parts of them that are no multiple of 16 elements (4096 rows of 9 + 3 heads of 72 7.0 us, the host's call and little more).
 template <bool SPLIT>
 __global__ __launch_bounds__(64 * kWaves) void rope_kernel(const RopeArgs a) {
     __shared__ float turn[kWaves][2 * kMostPairs];

@@ -128,7 +128,7 @@ int mi_rope(void* stream, const mi_rope_call* call);
  * With a window the earlier positions j are those with j > p - window or j < sinks, p = position[row] being the row's place in its
  * text (as for mi_rope; taken as no less than the number of earlier positions and less than kv_len); the bits alone
  * decide among new rows.  seen [n_tokens][words] and position [n_tokens]: device memory, 4-byte aligned; position may be null where
- * there is no window.  words 1 to 65536.  All else as mi_attention, whose kernels these are. */
+ * there is no window.  words 1 to 65536.  All else as mi_attention. */
 typedef struct mi_tree_mask {
     const unsigned* seen;
     const int* position;
