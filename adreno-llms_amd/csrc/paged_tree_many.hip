@@ -1,7 +1,8 @@
 // Attention of trees of many rows over a cache in pages (mi_attention_tree): the kernel for many rows, in a file of its own so that
-// both compile at the same time.  8 trees of 64 drafts behind 16384, 32 heads over 8 of width 128: fp16 108 us, int8 103, Q4 107.  What bounds it is the chain
+// both compile at the same time.  8 trees of 64 drafts behind 16384, 32 heads over 8 of width 128: fp16 108 us, int8 103, Q4 106.  What bounds it is the chain
 // of a tile, as in plain batches; counters of the fp16 ones: matrix cores busy 29 % of the SIMD-cycles, vector units 33 %, LDS 30 % of the CU-cycles (half of it
-// conflicts); of the wavefronts' time 40 % are instructions, 37 % waits for memory, LDS and barriers, 23 % for their turn.
+// conflicts); of the wavefronts' time 40 % are instructions, 37 % waits for memory, LDS and barriers, 23 % for their turn.  int8 and Q4, whose
+// tiles are converted on the way to LDS: 26 and 26 %, 40 and 45 %, 42 and 42 %; 39, 46 and 15 %, 39, 48 and 13 %.
 #include "paged_chunk.h"
 
 namespace mi {
